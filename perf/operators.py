@@ -426,7 +426,7 @@ def _plain_gate_train(s):
 # ------------------------------------------------------------------ the orthogonalised update, plain
 def _plain_orthogonal(u):
     norm = u.double().square().sum((1, 2), keepdim=True).sqrt()
-    x = torch.where(norm > 0, u / norm, 0.0).float()
+    x = torch.where(norm == 0, 0.0, u / norm).float()
     rows, cols = x.shape[1:]
     if rows > cols:
         x = x.transpose(1, 2).contiguous()
