@@ -134,6 +134,12 @@ SIGNATURES = {
     "bship_bias_act_f32": [c_int, _P, _P, _P, _I64, _I64],
     "bship_batchnorm_fwd_f32": [c_int, _P, _P, _P, _P, _P, c_double, c_double, _P, _P, _P, _P, _I64, _I64],
     "bship_batchnorm_bwd_f32": [_P] * 7 + [_I64, _I64],
+    "bship_linear_attention_fwd_f32": [_P] * 8 + [_I64] * 5 + [c_float],
+    "bship_linear_attention_bwd_f32": [_P] * 13 + [_I64] * 5 + [c_float],
+    "bship_gated_residual_fwd_f32": [c_int] + [_P] * 7 + [_I64] * 2 + [c_float] * 2,
+    "bship_gated_residual_bwd_f32": [c_int] + [_P] * 12 + [_I64] * 2 + [c_float] * 2 + [c_int],
+    "bship_orthogonalize_f32": [_P] * 2 + [_I64] * 3 + [c_int],
+    "bship_orthogonal_update_f32": [c_float, c_float, c_int] + [_P] * 3 + [_I64] * 3 + [c_int],
 }
 # functions that do not return a status
 SPECIAL_RESTYPES = {"bship_version": (c_int, []), "bship_last_error": (c_char_p, [])}

@@ -1,0 +1,531 @@
+// The norms around a block with its gate and residual scale, forward and backward, in one pass each:
+//
+//   y = residual_scale x + act(gate) * post * block / rms(block)        the norm behind the block, gate, residual
+//   h = pre * y / rms(y)                                                the norm before the next block
+//   rms(v) = sqrt(mean(v^2) + epsilon) over a row
+//
+// A row is read once, kept in registers and reduced there: 3 arrays in and 2 out forward, 5 in and 3 out
+// backward (the row's two means are formed again, which costs two reductions and no memory). The gate, the
+// second norm, and the block itself (only the norm: h = pre * x / rms(x)) can be left out.
+#include "common.h"
+
+#pragma clang fp contract(fast)
+
+namespace bship {
+namespace {
+
+struct GateArgs {
+    const float *block, *gate, *x, *post, *pre;    // gate NULL: 1; pre NULL: no norm behind; block NULL: y is x
+    float *y, *h;
+    const float *dy, *dh;                          // backward; y is read then
+    float *dblock, *dgate, *dx;
+    float* part;                                   // partial sums of the weights' gradients: (groups, 2, width)
+    int64_t rows;
+    int width;
+    int act;
+    float residual_scale, epsilon;
+    int accumulate;
+};
+
+__device__ __forceinline__ f4 load_row4(const float* p, int left) {
+    if (left >= 4) return *reinterpret_cast<const f4u*>(p);
+    f4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (left > 0) r[0] = p[0];
+    if (left > 1) r[1] = p[1];
+    if (left > 2) r[2] = p[2];
+    return r;
+}
+__device__ __forceinline__ void store_row4(float* p, f4 v, int left, bool add) {
+    if (left <= 0) return;
+    if (add) v += load_row4(p, left);
+    if (left >= 4) {
+        *reinterpret_cast<f4u*>(p) = v;
+        return;
+    }
+    p[0] = v[0];
+    if (left > 1) p[1] = v[1];
+    if (left > 2) p[2] = v[2];
+}
+
+__device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+// act(z), and its derivative by z
+__device__ __forceinline__ float gate_value(int act, float z) {
+    switch (act) {
+        case BSHIP_ACT_SIGMOID: return logistic(z);
+        case BSHIP_ACT_TANH:    return tanhf(z);
+        case BSHIP_ACT_REL:     return z > 0.0f || z != z ? z : 0.0f;
+        case BSHIP_ACT_EL:      return z > 0.0f ? z : expm1f(z);
+        case BSHIP_ACT_SWISH:   return z * logistic(z);
+        default:                return z;
+    }
+}
+__device__ __forceinline__ float gate_slope(int act, float z, float value) {
+    switch (act) {
+        case BSHIP_ACT_SIGMOID: return value * (1.0f - value);
+        case BSHIP_ACT_TANH:    return 1.0f - value * value;
+        case BSHIP_ACT_REL:     return z > 0.0f ? 1.0f : 0.0f;
+        case BSHIP_ACT_EL:      return z > 0.0f ? 1.0f : value + 1.0f;
+        case BSHIP_ACT_SWISH: {
+            const float s = logistic(z);
+            return s + value * (1.0f - s);
+        }
+        default:                return 1.0f;
+    }
+}
+
+// Sums over the TPR threads of a row (64: a wavefront, 256: the workgroup).
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* lds) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = wave_sum(v[n]);
+    if constexpr (TPR > kWave) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) lds[n * 4 + wave] = v[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = (lds[n * 4] + lds[n * 4 + 1]) + (lds[n * 4 + 2] + lds[n * 4 + 3]);
+        __syncthreads();
+    }
+}
+
+// TPR threads per row, V vectors of four floats per thread: width <= 4 TPR V.
+template <int TPR, int V>
+__global__ __launch_bounds__(kBlock) void gate_fwd_kernel(GateArgs a) {
+    __shared__ float lds[8];
+    constexpr int kRows = kBlock / TPR;
+    const int t = threadIdx.x % TPR;
+    const float inv_n = 1.0f / static_cast<float>(a.width);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; row < a.rows; row += step) {
+        const int64_t base = row * a.width;
+        f4 y[V];
+        if (a.block) {
+            f4 o[V], z[V];
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int m = 0; m < V; ++m) {
+                const int c = (t + m * TPR) * 4, left = a.width - c;
+                o[m] = load_row4(a.block + base + c, left);
+                y[m] = load_row4(a.x + base + c, left);
+                if (a.gate) z[m] = load_row4(a.gate + base + c, left);
+            }
+#pragma unroll
+            for (int m = 0; m < V; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[0] += o[m][r] * o[m][r];
+            row_sums<TPR>(s, lds);
+            const float rb = 1.0f / sqrtf(s[0] * inv_n + a.epsilon);
+#pragma unroll
+            for (int m = 0; m < V; ++m) {
+                const int c = (t + m * TPR) * 4, left = a.width - c;
+                const f4 w = load_row4(a.post + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float u = w[r] * (o[m][r] * rb);
+                    if (a.gate) u *= gate_value(a.act, z[m][r]);
+                    y[m][r] = a.residual_scale * y[m][r] + (r < left ? u : 0.0f);
+                }
+                store_row4(a.y + base + c, y[m], left, false);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < V; ++m) {
+                const int c = (t + m * TPR) * 4;
+                y[m] = load_row4(a.x + base + c, a.width - c);
+            }
+        }
+        if (!a.pre) continue;
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int m = 0; m < V; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[0] += y[m][r] * y[m][r];
+        row_sums<TPR>(s, lds);
+        const float ry = 1.0f / sqrtf(s[0] * inv_n + a.epsilon);
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            const int c = (t + m * TPR) * 4, left = a.width - c;
+            const f4 w = load_row4(a.pre + c, left);
+            store_row4(a.h + base + c, w * (y[m] * ry), left, false);
+        }
+    }
+}
+
+// Rows of any width: three passes over the row, the second and third mostly out of the caches.
+__global__ __launch_bounds__(kBlock) void gate_fwd_long_kernel(GateArgs a) {
+    __shared__ float lds[8];
+    const float inv_n = 1.0f / static_cast<float>(a.width);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t base = row * a.width;
+        const float* y = a.block ? a.y : a.x;
+        float s[1] = {0.0f};
+        if (a.block) {
+            for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+                const f4 o = load_row4(a.block + base + c, a.width - c);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[0] += o[r] * o[r];
+            }
+            row_sums<kBlock>(s, lds);
+            const float rb = 1.0f / sqrtf(s[0] * inv_n + a.epsilon);
+            s[0] = 0.0f;
+            for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+                const int left = a.width - c;
+                const f4 o = load_row4(a.block + base + c, left), w = load_row4(a.post + c, left);
+                f4 v = load_row4(a.x + base + c, left), z = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (a.gate) z = load_row4(a.gate + base + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float u = w[r] * (o[r] * rb);
+                    if (a.gate) u *= gate_value(a.act, z[r]);
+                    v[r] = a.residual_scale * v[r] + (r < left ? u : 0.0f);
+                    s[0] += v[r] * v[r];
+                }
+                store_row4(a.y + base + c, v, left, false);
+            }
+        } else {
+            for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+                const f4 v = load_row4(y + base + c, a.width - c);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[0] += v[r] * v[r];
+            }
+        }
+        if (!a.pre) continue;
+        row_sums<kBlock>(s, lds);
+        const float ry = 1.0f / sqrtf(s[0] * inv_n + a.epsilon);
+        for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {       // every thread reads what it wrote
+            const int left = a.width - c;
+            store_row4(a.h + base + c, load_row4(a.pre + c, left) * (load_row4(y + base + c, left) * ry), left, false);
+        }
+    }
+}
+
+// With e = dh * pre, n = block / rms(block):
+//   total = dy + (e - y mean(e y) / rms(y)^2) / rms(y)            what arrives at y
+//   dx = residual_scale total;  dgate = total post n act'(gate);  d = total post act(gate)
+//   dblock = (d - n mean(d n)) / rms(block);  dpost = sum total act(gate) n;  dpre = sum dh y / rms(y)
+// A workgroup keeps the columns' sums over its rows in registers (one row per TPR threads) or, for long rows, adds
+// them to its own row of `part`; they are added over the groups in a fixed order afterwards.
+template <int TPR, int V>
+__global__ __launch_bounds__(kBlock) void gate_bwd_kernel(GateArgs a) {
+    __shared__ float lds[12];
+    constexpr int kRows = kBlock / TPR;
+    const int t = threadIdx.x % TPR;
+    const float inv_n = 1.0f / static_cast<float>(a.width);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    f4 wpost[V], wpre[V], spost[V], spre[V];
+#pragma unroll
+    for (int m = 0; m < V; ++m) {
+        const int c = (t + m * TPR) * 4, left = a.width - c;
+        if (a.block) wpost[m] = load_row4(a.post + c, left);
+        if (a.pre) wpre[m] = load_row4(a.pre + c, left);
+        spost[m] = spre[m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; row < a.rows; row += step) {
+        const int64_t base = row * a.width;
+        f4 total[V], y[V], e[V], o[V], z[V];
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            const int c = (t + m * TPR) * 4, left = a.width - c;
+            total[m] = a.dy ? load_row4(a.dy + base + c, left) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (a.pre) {
+                y[m] = load_row4(a.y + base + c, left);
+                e[m] = load_row4(a.dh + base + c, left);
+            }
+            if (a.block) o[m] = load_row4(a.block + base + c, left);
+            if (a.gate) z[m] = load_row4(a.gate + base + c, left);
+        }
+        float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int m = 0; m < V; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (a.pre) {
+                    s[0] += y[m][r] * y[m][r];
+                    s[1] += e[m][r] * wpre[m][r] * y[m][r];
+                }
+                if (a.block) s[2] += o[m][r] * o[m][r];
+            }
+        row_sums<TPR>(s, lds);
+        if (a.pre) {
+            const float ry = 1.0f / sqrtf(s[0] * inv_n + a.epsilon), back = s[1] * inv_n * ry * ry;
+#pragma unroll
+            for (int m = 0; m < V; ++m) {
+                spre[m] += e[m] * (y[m] * ry);
+                total[m] += ry * (e[m] * wpre[m] - y[m] * back);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            const int c = (t + m * TPR) * 4;
+            store_row4(a.dx + base + c, a.residual_scale * total[m], a.width - c, a.accumulate);
+        }
+        if (!a.block) continue;
+        const float rb = 1.0f / sqrtf(s[2] * inv_n + a.epsilon);
+        float dn[1] = {0.0f};
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            const int c = (t + m * TPR) * 4, left = a.width - c;
+            f4 dz;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float n = o[m][r] * rb, value = a.gate ? gate_value(a.act, z[m][r]) : 1.0f;
+                const float tv = r < left ? total[m][r] * value : 0.0f;
+                if (a.gate) dz[r] = total[m][r] * (wpost[m][r] * n) * gate_slope(a.act, z[m][r], value);
+                spost[m][r] += tv * n;
+                total[m][r] = tv * wpost[m][r];                 // d from here on
+                dn[0] += total[m][r] * o[m][r];
+            }
+            if (a.gate) store_row4(a.dgate + base + c, dz, left, a.accumulate);
+        }
+        row_sums<TPR>(dn, lds);
+        const float back = dn[0] * inv_n * rb * rb;
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            const int c = (t + m * TPR) * 4;
+            store_row4(a.dblock + base + c, rb * (total[m] - o[m] * back), a.width - c, a.accumulate);
+        }
+    }
+    float* part = a.part + (static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR) * 2 * a.width;
+#pragma unroll
+    for (int m = 0; m < V; ++m) {
+        const int c = (t + m * TPR) * 4, left = a.width - c;
+        store_row4(part + c, spost[m], left, false);
+        store_row4(part + a.width + c, spre[m], left, false);
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void gate_bwd_long_kernel(GateArgs a) {
+    __shared__ float lds[12];
+    const float inv_n = 1.0f / static_cast<float>(a.width);
+    float* part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
+    for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+        store_row4(part + c, f4{0.0f, 0.0f, 0.0f, 0.0f}, a.width - c, false);
+        store_row4(part + a.width + c, f4{0.0f, 0.0f, 0.0f, 0.0f}, a.width - c, false);
+    }
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t base = row * a.width;
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+            const int left = a.width - c;
+            if (a.pre) {
+                const f4 y = load_row4(a.y + base + c, left);
+                const f4 e = load_row4(a.dh + base + c, left) * load_row4(a.pre + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[0] += y[r] * y[r];
+                    s[1] += e[r] * y[r];
+                }
+            }
+            if (a.block) {
+                const f4 o = load_row4(a.block + base + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[2] += o[r] * o[r];
+            }
+        }
+        row_sums<kBlock>(s, lds);
+        const float ry = 1.0f / sqrtf(s[0] * inv_n + a.epsilon), back_y = s[1] * inv_n * ry * ry;
+        const float rb = 1.0f / sqrtf(s[2] * inv_n + a.epsilon);
+        // what arrives at y, formed where it is needed; dx and dgate may be arrays that are read here only by the
+        // thread that writes them
+        auto total_of = [&](int c, int left) {
+            f4 v = a.dy ? load_row4(a.dy + base + c, left) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (a.pre)
+                v += ry * (load_row4(a.dh + base + c, left) * load_row4(a.pre + c, left) -
+                           load_row4(a.y + base + c, left) * back_y);
+            return v;
+        };
+        float dn[1] = {0.0f};
+        if (a.block)
+            for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+                const int left = a.width - c;
+                const f4 v = total_of(c, left), o = load_row4(a.block + base + c, left), w = load_row4(a.post + c, left);
+                f4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (a.gate) z = load_row4(a.gate + base + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < left) dn[0] += v[r] * (a.gate ? gate_value(a.act, z[r]) : 1.0f) * w[r] * o[r];
+            }
+        row_sums<kBlock>(dn, lds);
+        const float back_b = dn[0] * inv_n * rb * rb;
+        for (int c = threadIdx.x * 4; c < a.width; c += 4 * kBlock) {
+            const int left = a.width - c;
+            const f4 v = total_of(c, left);
+            if (a.pre)
+                store_row4(part + a.width + c,
+                           load_row4(a.dh + base + c, left) * (load_row4(a.y + base + c, left) * ry), left, true);
+            if (a.block) {
+                const f4 o = load_row4(a.block + base + c, left), w = load_row4(a.post + c, left);
+                f4 z = {0.0f, 0.0f, 0.0f, 0.0f}, dz, db, dw;
+                if (a.gate) z = load_row4(a.gate + base + c, left);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float n = o[r] * rb, value = a.gate ? gate_value(a.act, z[r]) : 1.0f;
+                    dz[r] = v[r] * (w[r] * n) * (a.gate ? gate_slope(a.act, z[r], value) : 0.0f);
+                    dw[r] = v[r] * value * n;
+                    db[r] = rb * (v[r] * value * w[r] - o[r] * back_b);
+                }
+                store_row4(part + c, dw, left, true);
+                if (a.gate) store_row4(a.dgate + base + c, dz, left, a.accumulate);
+                store_row4(a.dblock + base + c, db, left, a.accumulate);
+            }
+            store_row4(a.dx + base + c, a.residual_scale * v, left, a.accumulate);
+        }
+    }
+}
+
+// dpost[c], dpre[c] = the sum of the groups' parts: 64 columns per workgroup, its 16 rows of threads take every
+// 16th group.
+__global__ __launch_bounds__(1024) void gate_weights_kernel(const float* __restrict__ part, int64_t groups, int width,
+                                                            float* __restrict__ dpost, float* __restrict__ dpre) {
+    __shared__ float s[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+    float v = 0.0f;
+    if (c < 2 * width)
+        for (int64_t g = r; g < groups; g += 16) v += part[g * 2 * width + c];
+    s[r][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (r || c >= 2 * width) return;
+    v = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v += s[x][threadIdx.x];
+    if (c < width) {
+        if (dpost) dpost[c] = v;
+    } else if (dpre) {
+        dpre[c - width] = v;
+    }
+}
+
+constexpr int kLongWidth = 8192;        // wider rows do not stay in registers
+
+template <typename F>
+int by_width(int width, F&& f) {
+    if (width <= 256) return f.template operator()<64, 1>();
+    if (width <= 512) return f.template operator()<64, 2>();
+    if (width <= 1024) return f.template operator()<64, 4>();
+    if (width <= 2048) return f.template operator()<256, 2>();
+    if (width <= 4096) return f.template operator()<256, 4>();
+    return f.template operator()<256, 8>();
+}
+struct LaunchForward {
+    const GateArgs& a;
+    template <int TPR, int V> int operator()() const {
+        const unsigned grid = stream_grid(ceil_div(a.rows, kBlock / TPR));
+        hipLaunchKernelGGL((gate_fwd_kernel<TPR, V>), dim3(grid), dim3(kBlock), 0, ctx().stream, a);
+        return check_launch("gated_residual_forward");
+    }
+};
+struct LaunchBackward {
+    const GateArgs& a;
+    unsigned grid;
+    template <int TPR, int V> int operator()() const {
+        hipLaunchKernelGGL((gate_bwd_kernel<TPR, V>), dim3(grid), dim3(kBlock), 0, ctx().stream, a);
+        return check_launch("gated_residual_backward");
+    }
+};
+
+int check_arrays(const char* fn, const void* const* required, int count) {
+    for (int n = 0; n < count; ++n) {
+        if (!required[n]) return set_error(BSHIP_ERR_NULL_POINTER, "%s: a required array is NULL", fn);
+        if (reinterpret_cast<uintptr_t>(required[n]) & 3u)
+            return set_error(BSHIP_ERR_BAD_POINTER, "%s: an array is not 4-byte aligned", fn);
+    }
+    return 0;
+}
+int check_shape(const char* fn, int64_t rows, int64_t width, int act, bool gate) {
+    if (rows < 0 || width < 0 || width > (int64_t(1) << 28))
+        return set_error(BSHIP_ERR_BAD_DIMENSION, "%s: sizes out of range", fn);
+    if (gate && (act < BSHIP_ACT_SIGMOID || act > BSHIP_ACT_SWISH))
+        return set_error(BSHIP_ERR_BAD_OP, "%s: no activation has code %d", fn, act);
+    return 0;
+}
+
+}  // namespace
+}  // namespace bship
+
+using namespace bship;
+
+extern "C" {
+
+int bship_gated_residual_fwd_f32(int act, const float* block, const float* gate, const float* x, const float* post,
+                                 const float* pre, float* y, float* h, int64_t rows, int64_t width,
+                                 float residual_scale, float epsilon) {
+    BSHIP_REQUIRE_INIT();
+    int st = check_shape(__func__, rows, width, act, gate != nullptr);
+    if (st != 0) return st;
+    if (rows == 0 || width == 0) return 0;
+    GateArgs a = {};
+    a.block = block; a.gate = gate; a.x = x; a.post = post; a.pre = pre;
+    a.y = y; a.h = h;
+    a.rows = rows; a.width = static_cast<int>(width);
+    a.act = act; a.residual_scale = residual_scale; a.epsilon = epsilon;
+    const void* need[] = {x, block ? static_cast<const void*>(block) : x, block ? static_cast<const void*>(post) : x,
+                          block ? static_cast<const void*>(y) : x, pre ? static_cast<const void*>(h) : x,
+                          pre ? static_cast<const void*>(pre) : x, gate ? static_cast<const void*>(gate) : x};
+    if ((st = check_arrays(__func__, need, 7)) != 0) return st;
+    if (!block && (gate || !pre))
+        return set_error(BSHIP_ERR_NULL_POINTER, "%s: without a block there is only the norm before the next one", __func__);
+    if (width > kLongWidth) {
+        hipLaunchKernelGGL(gate_fwd_long_kernel, dim3(stream_grid(rows)), dim3(kBlock), 0, ctx().stream, a);
+        return check_launch("gated_residual_forward");
+    }
+    return by_width(a.width, LaunchForward{a});
+}
+
+int bship_gated_residual_bwd_f32(int act, const float* block, const float* gate, const float* post, const float* pre,
+                                 const float* y, const float* dy, const float* dh, float* dblock, float* dgate,
+                                 float* dx, float* dpost, float* dpre, int64_t rows, int64_t width,
+                                 float residual_scale, float epsilon, int accumulate) {
+    BSHIP_REQUIRE_INIT();
+    int st = check_shape(__func__, rows, width, act, gate != nullptr);
+    if (st != 0) return st;
+    if (width == 0) return 0;
+    if (rows == 0) {
+        if (dpost && (st = launch_fill(dpost, 0.0f, static_cast<size_t>(width))) != 0) return st;
+        return dpre ? launch_fill(dpre, 0.0f, static_cast<size_t>(width)) : 0;
+    }
+    if (!block && (gate || !pre))
+        return set_error(BSHIP_ERR_NULL_POINTER, "%s: without a block there is only the norm before the next one", __func__);
+    const void* need[] = {dx, block ? static_cast<const void*>(block) : dx, block ? static_cast<const void*>(post) : dx,
+                          block ? static_cast<const void*>(dblock) : dx, block ? static_cast<const void*>(dpost) : dx,
+                          gate ? static_cast<const void*>(gate) : dx, gate ? static_cast<const void*>(dgate) : dx,
+                          pre ? static_cast<const void*>(pre) : dx, pre ? static_cast<const void*>(y) : dx,
+                          pre ? static_cast<const void*>(dh) : dx, pre ? static_cast<const void*>(dpre) : dx,
+                          pre ? dx : static_cast<const void*>(dy), dy ? static_cast<const void*>(dy) : dx};
+    if ((st = check_arrays(__func__, need, 13)) != 0) return st;
+    GateArgs a = {};
+    a.block = block; a.gate = gate; a.post = post; a.pre = pre;
+    a.y = const_cast<float*>(y); a.dy = dy; a.dh = dh;
+    a.dblock = dblock; a.dgate = dgate; a.dx = dx;
+    a.rows = rows; a.width = static_cast<int>(width);
+    a.act = act; a.residual_scale = residual_scale; a.epsilon = epsilon;
+    a.accumulate = accumulate != 0;
+    // every group of threads that walks over rows leaves its part of the weights' gradients: few groups
+    const int per_block = width <= 1024 ? 4 : 1;
+    int64_t blocks = ceil_div(rows, per_block);
+    const int64_t most = 2 * static_cast<int64_t>(ctx().num_cus);
+    if (blocks > most) blocks = most;
+    void* part = nullptr;
+    st = pool_alloc_raw(static_cast<size_t>(blocks) * per_block * 2 * static_cast<size_t>(width) * sizeof(float), &part);
+    if (st != 0) return st;
+    a.part = static_cast<float*>(part);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    if (width > kLongWidth) {
+        hipLaunchKernelGGL(gate_bwd_long_kernel, dim3(grid), dim3(kBlock), 0, ctx().stream, a);
+        st = check_launch("gated_residual_backward");
+    } else {
+        st = by_width(a.width, LaunchBackward{a, grid});
+    }
+    if (st == 0) {
+        hipLaunchKernelGGL(gate_weights_kernel, dim3(static_cast<unsigned>(ceil_div(2 * width, 64))), dim3(1024), 0,
+                           ctx().stream, a.part, blocks * per_block, a.width, block ? dpost : nullptr,
+                           pre ? dpre : nullptr);
+        st = check_launch("gated_residual_backward, weights");
+    }
+    (void)pool_free_raw(part);
+    return st;
+}
+
+}  // extern "C"

@@ -272,6 +272,12 @@ class HipHandler(Handler):
         "momentum_update": ("velocity", "parameters"),
         "batchnorm_forward": ("mu", "sigma", "sigma_b", "centered", "x_hat", "out"),
         "batchnorm_backward": ("dgamma", "dbeta", "in_deltas"),
+        "linear_attention_forward": ("out", "new_state"), "linear_attention_step": ("state", "out"),
+        "linear_attention_backward": ("dq", "dk", "dv", "ddecay", "dstate"),
+        "gated_residual_forward": ("y", "h"), "rms_norm_forward": ("out",),
+        "gated_residual_backward": ("dblock", "dgate", "dx", "dpost_weight", "dpre_weight"),
+        "rms_norm_backward": ("dx", "dweight"),
+        "orthogonalize": ("out",), "orthogonal_update": ("velocity", "parameters"),
     }
 
     def _install_pitched_wrappers(self):
@@ -1374,3 +1380,180 @@ class HipHandler(Handler):
             raise ValueError("dropout_forward: inconsistent shapes")
         fn = self._lib.bship_dropout_fwd_fast_on_f32 if self.fast_masks else self._lib.bship_dropout_fwd_on_f32
         self._call(fn(self.rnd._id, inputs.ptr, mask.ptr, out.ptr, out.size, float(keep_probability), float(scale)))
+
+    # ----------------------------------- sequence, norm and update operators
+    @staticmethod
+    def _ptr(a):
+        return a.ptr if a is not None else None
+
+    @staticmethod
+    def _overlap(a, b):
+        """Whether two dense arrays share memory."""
+        return (a is not None and b is not None and a.size > 0 and b.size > 0
+                and a.ptr < b.ptr + b.nbytes and b.ptr < a.ptr + a.nbytes)
+
+    def _attention_shapes(self, op, q, k, v, decay, rows, states, lengths, others=()):
+        """(time, batch, heads, dk, dv) of a linear attention call whose q, k, v lead with the axes `rows`."""
+        heads = decay.size
+        lead = tuple(q.shape[:rows])
+        if len(q.shape) <= rows or q.shape != k.shape or len(v.shape) <= rows or tuple(v.shape[:rows]) != lead or not heads:
+            raise _mismatch(op, q, k, v, decay)
+        fk, fv = _prod(q.shape[rows:]), _prod(v.shape[rows:])
+        if fk % heads or fv % heads or not fk or not fv:
+            raise ValueError("%s: %d and %d features are not those of %d heads" % (op, fk, fv, heads))
+        time, batch = lead if rows == 2 else (1, lead[0])
+        dk, dv = fk // heads, fv // heads
+        if dk > 128 or dv > 128:
+            raise ValueError("%s: heads of %d and %d features; 128 are the most" % (op, dk, dv))
+        if any(s is not None and s.size != batch * heads * dk * dv for s in states):
+            raise ValueError("%s: a state must be %r" % (op, (batch, heads, dk, dv)))
+        if lengths is not None and lengths.size != batch:
+            raise _mismatch(op, q, lengths)
+        if any(a is not None and a.size != like.size for a, like in others):
+            raise _mismatch(op, *[a for a, _ in others if a is not None])
+        return time, batch, heads, dk, dv
+
+    def _no_overlap(self, op, outputs, inputs, allowed=()):
+        for n, a in enumerate(outputs):
+            for b in list(inputs) + list(outputs[n + 1:]):
+                if self._overlap(a, b) and not any(a is x and b is y for x, y in allowed):
+                    raise ValueError("%s: an output overlaps another operand" % op)
+
+    def linear_attention_forward(self, q, k, v, decay, out, scale=1.0, state=None, new_state=None, lengths=None):
+        """Linear attention with a decay for each head over a whole sequence: S_t = decay S_(t-1) + k_t^T v_t,
+        out_t = scale q_t S_t. q, k are (time, batch, heads * dk), v and out (time, batch, heads * dv), decay
+        (heads), dk and dv at most 128. state (batch, heads, dk, dv) is S before the first step (None: zeros),
+        new_state receives S behind the last one and may be state. lengths (batch elements, like labels) gives
+        the steps of each: rows from there on are not read, out is 0 there."""
+        sizes = self._attention_shapes("linear_attention_forward", q, k, v, decay, 2, (state, new_state), lengths,
+                                       ((out, v),))
+        shared = ((new_state, state),) if new_state is not None and state is not None and new_state.ptr == state.ptr else ()
+        self._no_overlap("linear_attention_forward", [out, new_state], [q, k, v, decay, state, lengths], shared)
+        self._call(self._lib.bship_linear_attention_fwd_f32(
+            q.ptr, k.ptr, v.ptr, decay.ptr, self._ptr(lengths), self._ptr(state), out.ptr, self._ptr(new_state),
+            *sizes, scale))
+
+    def linear_attention_step(self, q, k, v, decay, state, out, scale=1.0):
+        """One step of linear_attention_forward: q, k are (batch, heads * dk), v and out (batch, heads * dv), and
+        state (batch, heads, dk, dv) is replaced by its successor."""
+        sizes = self._attention_shapes("linear_attention_step", q, k, v, decay, 1, (state,), None, ((out, v),))
+        self._no_overlap("linear_attention_step", [out, state], [q, k, v, decay])
+        self._call(self._lib.bship_linear_attention_fwd_f32(
+            q.ptr, k.ptr, v.ptr, decay.ptr, None, state.ptr, out.ptr, state.ptr, *sizes, scale))
+
+    def linear_attention_backward(self, q, k, v, decay, dout, dq, dk, dv, ddecay=None, scale=1.0, state=None,
+                                  dnew_state=None, dstate=None, lengths=None):
+        """The gradients of linear_attention_forward with the same q, k, v, decay, scale, state and lengths:
+        dout and dnew_state (None: zeros) are those of out and new_state; dq, dk, dv, ddecay and dstate (the last
+        two None: not wanted) are overwritten. dstate may be dnew_state."""
+        op = "linear_attention_backward"
+        sizes = self._attention_shapes(op, q, k, v, decay, 2, (state, dnew_state, dstate), lengths,
+                                       ((dout, v), (dq, q), (dk, k), (dv, v), (ddecay, decay)))
+        shared = (((dstate, dnew_state),) if dstate is not None and dnew_state is not None
+                  and dstate.ptr == dnew_state.ptr else ())
+        self._no_overlap(op, [dq, dk, dv, ddecay, dstate], [q, k, v, decay, dout, state, dnew_state, lengths], shared)
+        self._call(self._lib.bship_linear_attention_bwd_f32(
+            q.ptr, k.ptr, v.ptr, decay.ptr, self._ptr(lengths), self._ptr(state), dout.ptr, self._ptr(dnew_state),
+            dq.ptr, dk.ptr, dv.ptr, self._ptr(ddecay), self._ptr(dstate), *sizes, scale))
+
+    _GATE_CODES = dict(_ACT_CODES, swish=5)
+
+    def _gate_code(self, op, activation):
+        code = self._GATE_CODES.get(activation)
+        if code is None:
+            raise ValueError("%s: no activation is called %r" % (op, activation))
+        return code
+
+    def gated_residual_forward(self, activation, block, gate, x, post_weight, pre_weight, y, h, residual_scale=1.0,
+                               epsilon=1e-6):
+        """y = residual_scale * x + act(gate) * post_weight * block / rms(block) and h = pre_weight * y / rms(y), the
+        norms behind a block and before the next one with the block's gate, in one pass. Matrices are
+        (rows, width), weights have width elements, rms(v) = sqrt(mean(v * v) + epsilon) over a row. gate may
+        be None (no gate), pre_weight and h together (no norm behind). Activations: those of act_func and
+        'swish'."""
+        code = self._gate_code("gated_residual_forward", activation)
+        self._gate_shapes("gated_residual_forward", (block, x, y), (gate,), (post_weight,), pre_weight, (h,))
+        rows, width = x.shape
+        self._call(self._lib.bship_gated_residual_fwd_f32(
+            code, block.ptr, self._ptr(gate), x.ptr, post_weight.ptr, self._ptr(pre_weight),
+            y.ptr, self._ptr(h), rows, width, residual_scale, epsilon))
+
+    def gated_residual_backward(self, activation, block, gate, post_weight, pre_weight, y, dy, dh, dblock, dgate, dx,
+                                dpost_weight, dpre_weight, residual_scale=1.0, epsilon=1e-6, accumulate=True):
+        """The gradients of gated_residual_forward. dblock, dgate and dx are added to what they hold (as a layer
+        adds to its input deltas) or, with accumulate=False, overwritten; the weights' gradients are
+        overwritten. gate and dgate are None together, and so are pre_weight, dh and dpre_weight."""
+        op = "gated_residual_backward"
+        code = self._gate_code(op, activation)
+        self._gate_shapes(op, (block, dy, dblock, dx), (gate, dgate), (post_weight, dpost_weight), pre_weight,
+                          (y, dh), (dpre_weight,))
+        if (gate is None) != (dgate is None):
+            raise ValueError("%s: gate and dgate go together" % op)
+        rows, width = dx.shape
+        self._call(self._lib.bship_gated_residual_bwd_f32(
+            code, block.ptr, self._ptr(gate), post_weight.ptr, self._ptr(pre_weight),
+            self._ptr(y), dy.ptr, self._ptr(dh) if pre_weight is not None else None, dblock.ptr, self._ptr(dgate),
+            dx.ptr, dpost_weight.ptr, self._ptr(dpre_weight), rows, width, residual_scale, epsilon,
+            int(bool(accumulate))))
+
+    @staticmethod
+    def _gate_shapes(op, matrices, optional, weights, pre_weight, pre_matrices, pre_weights=()):
+        """Every matrix (rows, width), every weight of width elements; what belongs to the second norm is there
+        exactly if its weight is."""
+        shape = matrices[0].shape
+        if len(shape) != 2:
+            raise ValueError("%s: matrices are wanted, got %r" % (op, tuple(shape)))
+        given = [m for m in optional if m is not None]
+        vectors = list(weights)
+        if pre_weight is not None:
+            if any(m is None for m in tuple(pre_matrices) + tuple(pre_weights)):
+                raise ValueError("%s: an operand of the norm before the next block is missing" % op)
+            given += pre_matrices
+            vectors += [pre_weight] + list(pre_weights)
+        if any(m.shape != shape for m in list(matrices) + given) or any(w.size != shape[1] for w in vectors):
+            raise _mismatch(op, *(list(matrices) + given + vectors))
+
+    def rms_norm_forward(self, x, weight, out, epsilon=1e-6):
+        """out = weight * x / sqrt(mean(x * x) + epsilon) over the rows of a (rows, width) matrix: the norm before the
+        first block."""
+        self._gate_shapes("rms_norm_forward", (x, out), (), (weight,), None, ())
+        rows, width = x.shape
+        self._call(self._lib.bship_gated_residual_fwd_f32(3, None, None, x.ptr, None, weight.ptr, None, out.ptr, rows,
+                                                          width, 1.0, epsilon))
+
+    def rms_norm_backward(self, x, weight, dout, dx, dweight, epsilon=1e-6, accumulate=True):
+        """The gradients of rms_norm_forward; dx is added to what it holds or, with accumulate=False, overwritten,
+        dweight is overwritten."""
+        self._gate_shapes("rms_norm_backward", (x, dout, dx), (), (weight, dweight), None, ())
+        rows, width = x.shape
+        self._call(self._lib.bship_gated_residual_bwd_f32(3, None, None, None, weight.ptr, x.ptr, None, dout.ptr, None,
+                                                          None, dx.ptr, None, dweight.ptr, rows, width, 1.0, epsilon,
+                                                          int(bool(accumulate))))
+
+    @staticmethod
+    def _matrices(op, a):
+        """(count, rows, cols) of a matrix or of a stack of equal matrices."""
+        if len(a.shape) not in (2, 3):
+            raise ValueError("%s: a matrix or a stack of matrices is wanted, got %r" % (op, tuple(a.shape)))
+        return (1,) * (3 - len(a.shape)) + tuple(a.shape)
+
+    def orthogonalize(self, m, out, steps=5):
+        """out = the matrix m, or each of a stack (count, rows, cols), with its singular values brought to about 1 by
+        `steps` Newton-Schulz steps. out may be m."""
+        if out.shape != m.shape:
+            raise _mismatch("orthogonalize", m, out)
+        count, rows, cols = self._matrices("orthogonalize", m)
+        if out.ptr != m.ptr:
+            self._no_overlap("orthogonalize", [out], [m])
+        self._call(self._lib.bship_orthogonalize_f32(m.ptr, out.ptr, count, rows, cols, steps))
+
+    def orthogonal_update(self, momentum, neg_learning_rate, gradients, velocity, parameters, steps=5, nesterov=True):
+        """velocity = momentum * velocity + gradients; parameters += neg_learning_rate * sqrt(max(1, rows / cols)) *
+        orthogonalize(gradients + momentum * velocity, or velocity without nesterov), for one matrix or a stack of
+        equal ones (count, rows, cols): momentum_update for weight matrices."""
+        if not (gradients.shape == velocity.shape == parameters.shape):
+            raise _mismatch("orthogonal_update", gradients, velocity, parameters)
+        count, rows, cols = self._matrices("orthogonal_update", parameters)
+        self._no_overlap("orthogonal_update", [velocity, parameters], [gradients])
+        self._call(self._lib.bship_orthogonal_update_f32(momentum, neg_learning_rate, int(bool(nesterov)), gradients.ptr,
+                                                         velocity.ptr, parameters.ptr, count, rows, cols, steps))

@@ -519,7 +519,8 @@ enum {
     BSHIP_ACT_TANH = 1,
     BSHIP_ACT_REL = 2,
     BSHIP_ACT_LINEAR = 3,
-    BSHIP_ACT_EL = 4
+    BSHIP_ACT_EL = 4,
+    BSHIP_ACT_SWISH = 5 /* z sigmoid(z): the gate of bship_gated_residual_* only */
 };
 /* LstmLayerImpl.forward_pass, the part of the loop body after the four
  * dot_add_mm calls (lstm_layer.py 121-145). Za, Ia, Fa, Oa hold the
@@ -696,6 +697,73 @@ int bship_fusing_flush(void);
 int bship_fusing_stats(unsigned long long* calls, unsigned long long* unfused,
                        unsigned long long* fused_calls, unsigned long long* fused_launches,
                        unsigned long long* overtaken, int reset);
+
+/* ----------------------- sequence, norm and update operators ----------------------- */
+
+/* Linear attention with a decay for each head, a recurrent layer's whole sequence:
+ *     S_t = decay[h] S_(t-1) + k_t^T v_t,    out_t = scale q_t S_t
+ * for every batch element and head. q, k are (time, batch, heads * dk), v and out (time, batch,
+ * heads * dv), a head's features side by side; decay is (heads), any finite values (0 keeps the
+ * position itself only, 1 forgets nothing); state, S before the first step, is (batch, heads, dk, dv)
+ * or NULL for zeros; new_state receives S behind the last step (NULL: not wanted) and may be state.
+ * lengths (batch) or NULL: the steps of each batch element, float32 like all labels, truncated and
+ * taken into [0, time] (NaN: 0); rows at and behind a length are neither read nor added to the state,
+ * and out is 0 there. dk and dv are 1 to 128, else BSHIP_ERR_UNSUPPORTED with nothing launched.
+ * A value that is not finite reaches the outputs of its own and later positions only. out may not
+ * overlap an input. Products and sums are float32. Takes scratch from the pool; recordable. */
+int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* v,
+                                   const float* decay, const float* lengths, const float* state,
+                                   float* out, float* new_state, int64_t time, int64_t batch,
+                                   int64_t heads, int64_t dk, int64_t dv, float scale);
+/* Its gradients: dq, dk_out, dv_out (shaped like q, k, v; 0 in rows behind a length), ddecay (heads;
+ * NULL: not wanted), dstate (like state; NULL: not wanted), all overwritten. dout is the gradient of
+ * out, dnew_state that of new_state or NULL for zeros; dstate may be dnew_state, no other output may
+ * overlap an input. The sums are in a fixed order: the same bits every time. */
+int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* v,
+                                   const float* decay, const float* lengths, const float* state,
+                                   const float* dout, const float* dnew_state, float* dq,
+                                   float* dk_out, float* dv_out, float* ddecay, float* dstate,
+                                   int64_t time, int64_t batch, int64_t heads, int64_t dk,
+                                   int64_t dv, float scale);
+
+/* The norms around a block with its gate and residual scale, over (rows, width) matrices:
+ *     y = residual_scale x + act(gate) * post * block / rms(block),    h = pre * y / rms(y),
+ *     rms(v) = sqrt(mean(v * v) + epsilon) over a row
+ * act is a BSHIP_ACT_* code, BSHIP_ACT_SWISH included. gate NULL: no gate. pre NULL: no norm behind, h
+ * is not written. block NULL: only the norm, h = pre * x / rms(x), y is not written. An output may be
+ * one of the inputs. Recordable. */
+int bship_gated_residual_fwd_f32(int act, const float* block, const float* gate, const float* x,
+                                 const float* post, const float* pre, float* y, float* h,
+                                 int64_t rows, int64_t width, float residual_scale,
+                                 float epsilon);
+/* Its gradients, from dy and dh (those of y and h; dy may be NULL if pre is given, dh is not read if
+ * pre is NULL). dblock, dgate, dx are added to what they hold if accumulate is not 0 (as a layer's
+ * backward pass adds to its input deltas), else overwritten, and may then be one of the inputs;
+ * dpost and dpre (width) are overwritten, summed over the rows in a fixed order. y is the forward
+ * pass's y (its x if block is NULL); it is not read if pre is NULL. Takes scratch from the pool;
+ * recordable. */
+int bship_gated_residual_bwd_f32(int act, const float* block, const float* gate,
+                                 const float* post, const float* pre, const float* y,
+                                 const float* dy, const float* dh, float* dblock, float* dgate,
+                                 float* dx, float* dpost, float* dpre, int64_t rows,
+                                 int64_t width, float residual_scale, float epsilon,
+                                 int accumulate);
+
+/* out = in / |in|_F after `steps` (1 to 100) Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T,
+ * (a, b, c) = (3.4445, -4.7750, 2.0315), for each of `count` matrices (rows, cols) back to back: the
+ * singular values go to about 1 and the singular vectors stay. A matrix of zeros stays one; one with
+ * a NaN or an infinity becomes NaN. out may be in. Products are taken from 22-bit splits of the
+ * float32 values with float32 sums. Takes scratch from the pool (16 bytes per entry and 8 per entry of
+ * the square of the smaller side, sides rounded up to 128); recordable. */
+int bship_orthogonalize_f32(const float* in, float* out, int64_t count, int64_t rows, int64_t cols,
+                            int steps);
+/* A momentum update whose matrices are orthogonalised: velocity = momentum * velocity + gradients;
+ * u = gradients + momentum * velocity (nesterov not 0) or velocity;
+ * parameters += neg_learning_rate * sqrt(max(1, rows / cols)) * orthogonalised u.
+ * The three arrays hold `count` matrices (rows, cols) and may not overlap. */
+int bship_orthogonal_update_f32(float momentum, float neg_learning_rate, int nesterov,
+                                const float* gradients, float* velocity, float* parameters,
+                                int64_t count, int64_t rows, int64_t cols, int steps);
 
 #ifdef __cplusplus
 }
