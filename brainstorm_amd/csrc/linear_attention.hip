@@ -35,6 +35,9 @@ namespace bship {
 namespace {
 
 constexpr int kChunk = 32;
+constexpr int64_t kStepFloats = int64_t(1) << 25;      // batch * heads * d of a pass: 31 rows within 4 GiB
+constexpr int kAddedUp = 4;       // up to so many segments a pass adds up what the ones before leave by itself; the scan of
+                                  // more is a launch of its own (1024 steps, 128 sequences of 128 features: 685 us with, 760 without)
 constexpr int kStepMost = 4;      // sequences of at most this many positions go position by position
 
 struct PassArgs {
@@ -46,11 +49,12 @@ struct PassArgs {
     const float* z;                    // TAN: the array of o's shape that the derivative of o by g is multiplied with
     const float* dfin;                 // TAN: gradient of the final state (strides si, sj), or NULL
     double* slope;                     // TAN: one partial sum per workgroup
-    float* seg;                        // states at the beginning of each segment: (batch*heads, segs, 1 or 2, di, dj)
+    float* seg;                        // what each segment leaves, or starts from: (batch*heads, segs, 1 or 2, di, dj)
     int64_t time, batch, heads;
     int di, dj, si, sj;
     int segs, seg_len;                 // segments of seg_len positions (a multiple of kChunk)
-    int tiles_j;                       // workgroups that share the columns of one head
+    int scanned;                       // `seg` holds the states that segments start from, not what they leave
+    int tiles_j;                       // single steps: workgroups that share the columns of one head
     float kv_scale, out_scale;
     int reverse;
 };
@@ -97,378 +101,745 @@ __device__ __forceinline__ void store4(float* p, f4 x, int left) {
 // scores never leave their layout.
 __device__ __forceinline__ f4 mfma(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// NI: tiles of 16 features of q and k held (di <= 16 NI); NJ: tiles of 16 features of v per wavefront (a
-// workgroup of four wavefronts has 64 NJ of them); TAN: with the derivative by the decay; STATE: only the
-// state behind a segment that starts from zero.
-template <int NI, int NJ, bool TAN, bool STATE>
-__global__ __launch_bounds__(kBlock) void la_pass_kernel(PassArgs a) {
-    constexpr int LD = 16 * NI + 4;        // rows of q and k in LDS: 4 floats longer, so that 16 lanes in 16 rows and
-    constexpr int LDV = 64 * NJ + 4;       // 64 lanes in 4 x 16 floats of rows 4 apart each meet 64 banks
-    __shared__ float q_s[STATE ? 4 : kChunk * LD];
-    __shared__ float k_s[kChunk * LD];
-    __shared__ float v_s[kChunk * LDV];
-    __shared__ f4 score_s[STATE ? 1 : (TAN ? 6 : 3) * kWave];
-    __shared__ float pw[kChunk + 1], sl[kChunk + 1];     // g^n and n g^(n-1)
-    __shared__ double part_s[4];
+// Keeps what is written before this point before it: the next step's LDS reads then are under way during this step's
+// products, and not all of them at once, each in registers of its own.
+__device__ __forceinline__ void one_step_ahead() { __builtin_amdgcn_sched_barrier(0); }
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// x, but the compiler does not know: what is formed from it is formed where it is used, a few instructions each time,
+// and does not stay in registers through the loop over the chunks.
+__device__ __forceinline__ int form_again(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Several passes over the same sequences in one launch (blockIdx.y): more workgroups at once, one tail.
+struct Passes {
+    PassArgs pass[2];
+};
+
+// NI: tiles of 16 features of q and k held (di <= 16 NI). NW: wavefronts, each with 16 features of v (dj <= 16 NW). TAN:
+// with the derivative by the decay. STATE: only the state behind a segment that starts from zero.
+//
+// q and k of a chunk are staged in LDS (every wavefront reads all of both, as operands of the scores, of q C and of
+// the state's update), fetched into registers one chunk ahead; v, which a wavefront needs only its own columns of, goes
+// from memory into the operand registers directly. Scores are shared through LDS in the layout that the product with
+// v takes them in. Per chunk and wavefront 8 NI + 8 NI + 12 + 3 NI / 2 (NW = 8) matrix instructions: the float32
+// matrix rate is what bounds the pass at 128 features, memory at 64 and below.
+template <int NI, int NW, bool TAN, bool STATE, bool NARROW>
+__global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : TAN ? 3 : 4) void la_pass_kernel(Passes passes) {
+    constexpr int LD = 16 * NI + 4;        // rows in LDS are 4 floats longer: 16 lanes in 16 rows, and 64 lanes in 16
+                                           // floats each of rows 4 apart, meet all 64 banks
+    constexpr int kThreads = NW * kWave;
+    constexpr int kRows = kChunk * LD;
+    __shared__ __attribute__((aligned(16))) float q_all[STATE ? 4 : 2 * kRows];
+    __shared__ __attribute__((aligned(16))) float k_all[2 * kRows];
+    __shared__ f4 score_s[STATE ? 1 : (TAN ? 6 : 3) * kWave];
+    __shared__ float pw[kChunk + 1], pl[kChunk + 1], sl[kChunk + 1];     // g^n, what its rounding left, n g^(n-1)
+    __shared__ float pk[kChunk + 1], sk[kChunk + 1];                     // kv_scale times g^n and n g^(n-1)
+    __shared__ double part_s[NW];
+
+    const PassArgs& a = passes.pass[blockIdx.y];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lq = lane >> 4;
-    const int jt0 = static_cast<int>(blockIdx.x % a.tiles_j) * 64 * NJ;
-    const int64_t rest = blockIdx.x / a.tiles_j;
-    const int seg = static_cast<int>(rest % a.segs);
+    const int seg = static_cast<int>(blockIdx.x % a.segs);
     if (STATE && seg + 1 == a.segs) return;               // nothing starts behind the last segment
-    const int64_t bh = rest / a.segs, b = bh / a.heads, h = bh % a.heads;
+    const int64_t bh = blockIdx.x / a.segs, b = bh / a.heads, h = bh % a.heads;
     const int64_t len = sequence_length(a.lengths, b, a.time);
     const int64_t p0 = static_cast<int64_t>(seg) * a.seg_len;
     const int64_t p1 = p0 + a.seg_len < a.time ? p0 + a.seg_len : a.time;
     const int64_t pe = len < p1 ? (len > p0 ? len : p0) : p1;      // valid positions [p0, pe)
     const double g = a.decay[h];
     const float gf = a.decay[h];
-    const int ni = (a.di + 15) >> 4;
-    const int dj = a.dj - jt0;                                     // columns from this workgroup's first on
+    const int j0 = 16 * wave;                                      // this wavefront's columns
+    const bool mine = j0 < a.dj;
 
+    // Position p is time p forwards, len - 1 - p backwards. Rows are addressed from a chunk's earliest time, which is
+    // the same for all lanes, by a 32-bit byte offset (a chunk spans less than 4 GiB: run_passes). Loads are made
+    // without conditions, so that the ones of a chunk are all under way at once: positions, pieces and columns that do
+    // not exist are taken from ones that do, and replaced by zeros or left out further on.
     const int64_t step_i = a.batch * a.heads * a.di, step_j = a.batch * a.heads * a.dj;
-    const float* q = a.q + bh * a.di;
-    const float* k = a.k + bh * a.di;
-    const float* v = a.v + bh * a.dj + jt0;
-
-    if (tid <= kChunk) {
-        pw[tid] = static_cast<float>(power(g, tid));
-        sl[tid] = tid ? static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
-    }
-
-    // ---- the state: tile (it, jt) of this wavefront's columns 16 (4 jt + wave) .. + 15
-    f4 c[NI][NJ], dc[TAN ? NI : 1][NJ];
-    const int64_t per_state = static_cast<int64_t>(a.di) * a.dj;
-#pragma unroll
-    for (int it = 0; it < NI; ++it)
-#pragma unroll
-        for (int jt = 0; jt < NJ; ++jt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * it + 4 * lq + r, j = 16 * (4 * jt + wave) + l16;
-                float x = 0.0f, dx = 0.0f;
-                if (!STATE && i < a.di && j < dj) {
-                    if (a.segs > 1) {
-                        const float* s = a.seg + (bh * a.segs + seg) * per_state * (TAN ? 2 : 1) +
-                                         static_cast<int64_t>(i) * a.dj + jt0 + j;
-                        x = s[0];
-                        if (TAN) dx = s[per_state];
-                    } else if (a.init) {
-                        const float s = a.init[bh * per_state + static_cast<int64_t>(i) * a.si +
-                                               static_cast<int64_t>(jt0 + j) * a.sj];
-                        x = len > 0 && !a.reverse ? gf * s : s;
-                        if (TAN) dx = len > 0 ? s : 0.0f;
-                    }
-                }
-                c[it][jt][r] = x;
-                if (TAN) dc[it][jt][r] = dx;
-            }
-    double slope = 0.0;
+    const int64_t t0 = a.reverse ? len - 1 - p0 - (kChunk - 1) : p0;
+    const int64_t move_i = (a.reverse ? -kChunk : kChunk) * step_i, move_j = (a.reverse ? -kChunk : kChunk) * step_j;
+    const float *q = a.q + t0 * step_i + bh * a.di, *k = a.k + t0 * step_i + bh * a.di;
+    const float* v = a.v + t0 * step_j + bh * a.dj + (mine ? j0 : 0);
+    float* out = a.out + t0 * step_j + bh * a.dj + j0;
+    const float* z = TAN ? a.z + t0 * step_j + bh * a.dj + j0 : nullptr;
+    const uint32_t step_i32 = static_cast<uint32_t>(step_i) * 4, step_j32 = static_cast<uint32_t>(step_j) * 4;
+    auto row_offset = [&](int row, uint32_t step) { return static_cast<uint32_t>(a.reverse ? kChunk - 1 - row : row) * step; };
+    auto at_offset = [](const float* p, uint32_t offset) {
+        return reinterpret_cast<const float*>(reinterpret_cast<const char*>(p) + offset);
+    };
+    constexpr int kRowQ = 4 * NI, kPieces = kChunk * kRowQ;              // 16-byte pieces of a row, of a chunk
+    constexpr int kLoads = (kPieces + kThreads - 1) / kThreads;
+    // column of piece e: the last one of a row whose length is no multiple of 4 ends with the row
+    auto piece_col = [&](int e) {
+        const int col = e % kRowQ * 4;
+        return NARROW || col >= a.di ? 0 : col + 4 > a.di ? a.di - 4 : col;
+    };
 
     // ---- rows of the next chunk, on their way from memory
-    constexpr int kRowQ = 4 * NI, kRowV = 16 * NJ;                       // 16-byte pieces of a row
-    constexpr int kLoadQ = kChunk * kRowQ / kBlock, kLoadV = kChunk * kRowV / kBlock;
-    static_assert(kChunk * kRowQ % kBlock == 0 && kChunk * kRowV % kBlock == 0, "whole pieces per thread");
-    f4 q_n[STATE ? 1 : kLoadQ], k_n[kLoadQ], v_n[kLoadV];
-    auto time_of = [&](int64_t p) { return a.reverse && p < len ? len - 1 - p : p; };
-    auto fetch = [&](int64_t pc) {
+    f4 q_n[STATE ? 1 : kLoads], k_n[kLoads];
+    float v_n[2][4];
+    // Pieces of one thread that lie in one column differ by whole rows; so do the rows of v. Their distances are scalars.
+    constexpr bool kColumn = kThreads % kRowQ == 0;
+    const uint32_t turn_j = a.reverse ? 0u - step_j32 : step_j32;
+    const uint32_t turn_i = (a.reverse ? 0u - step_i32 : step_i32) * (kThreads / kRowQ);
+    const uint32_t first_q = row_offset(tid / kRowQ % kChunk, step_i32) + 4 * piece_col(tid);
+    const uint32_t first_v = row_offset(4 * lq, step_j32) + 4 * (l16 < a.dj - j0 ? l16 : 0);
+    auto fetch = [&](int n) {                                            // the n positions of the chunk at q, k, v
+        uint32_t off_q[kLoads], off_v[2][4];
+        if (n == kChunk && kColumn && kPieces >= kThreads) {
 #pragma unroll
-        for (int m = 0; m < kLoadQ; ++m) {
-            const int e = tid + m * kBlock, row = e / kRowQ, col = e % kRowQ * 4;
-            const int64_t p = pc + row;
-            const bool valid = p < pe && col < a.di;
-            const int64_t at = valid ? time_of(p) * step_i + col : 0;
-            const int left = valid ? a.di - col : 0;
-            if (!STATE) q_n[m] = load4(q + at, left);
-            k_n[m] = load4(k + at, left);
+            for (int m = 0; m < kLoads; ++m) off_q[m] = first_q + m * turn_i;
+#pragma unroll
+            for (int bt = 0; bt < 2; ++bt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) off_v[bt][r] = first_v + (16 * bt + r) * turn_j;
+        } else {
+            const int tid = form_again(threadIdx.x), l16 = tid & 15, lq = tid >> 4 & 3;
+#pragma unroll
+            for (int m = 0; m < kLoads; ++m) {
+                const int row = (tid + m * kThreads) / kRowQ % kChunk;
+                off_q[m] = row_offset(row < n ? row : n - 1, step_i32) + 4 * piece_col(tid + m * kThreads);
+            }
+#pragma unroll
+            for (int bt = 0; bt < 2; ++bt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * bt + 4 * lq + r;
+                    off_v[bt][r] = row_offset(row < n ? row : n - 1, step_j32) + 4 * (l16 < a.dj - j0 ? l16 : 0);
+                }
         }
 #pragma unroll
-        for (int m = 0; m < kLoadV; ++m) {
-            const int e = tid + m * kBlock, row = e / kRowV, col = e % kRowV * 4;
-            const int64_t p = pc + row;
-            const bool valid = p < pe && col < dj;
-            v_n[m] = load4(v + (valid ? time_of(p) * step_j + col : 0), valid ? dj - col : 0);
+        for (int m = 0; m < kLoads; ++m) {
+            if constexpr (NARROW) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t at = off_q[m] + 4 * (r < a.di ? r : 0);
+                    k_n[m][r] = *at_offset(k, at);
+                    if (!STATE) q_n[m][r] = *at_offset(q, at);
+                }
+            } else {
+                k_n[m] = *reinterpret_cast<const f4u*>(at_offset(k, off_q[m]));
+                if (!STATE) q_n[m] = *reinterpret_cast<const f4u*>(at_offset(q, off_q[m]));
+            }
         }
+#pragma unroll
+        for (int bt = 0; bt < 2; ++bt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v_n[bt][r] = *at_offset(v, off_v[bt][r]);
     };
-    fetch(p0);
+    const auto positions = [&](int64_t pc) {                             // of the chunk pc behind p0
+        return pe - p0 - pc < kChunk ? static_cast<int>(pe - p0 - pc) : kChunk;
+    };
+    if (p0 < pe) fetch(positions(0));
+    // columns that a row does not have: zeros, which nothing overwrites
+    for (int e = tid * 4; e < 2 * kRows; e += kThreads * 4) {
+        *reinterpret_cast<f4*>(k_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!STATE) *reinterpret_cast<f4*>(q_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
-    for (int64_t pc = p0; pc < pe; pc += kChunk) {
-        const int n = pe - pc < kChunk ? static_cast<int>(pe - pc) : kChunk;
+    if (tid <= kChunk) {
+        const double x = power(g, tid);
+        pw[tid] = static_cast<float>(x);
+        pl[tid] = static_cast<float>(x - pw[tid]);
+        sl[tid] = tid ? static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
+        pk[tid] = a.kv_scale * pw[tid];
+        sk[tid] = a.kv_scale * sl[tid];
+    }
+
+    // ---- the state: rows 16 it + 4 lq + r, column j0 + l16
+    f4 c[NI], dc[TAN ? NI : 1];
+    const int64_t per_state = static_cast<int64_t>(a.di) * a.dj;
+    {
+        const float *from = nullptr, *dfrom = nullptr;
+        int row = a.si, column = a.sj;
+        const int64_t each = per_state * (TAN ? 2 : 1);
+        const float* slots = a.seg + bh * a.segs * each;             // not used with one segment
+        if (!STATE && a.scanned) {
+            from = slots + seg * each;
+            dfrom = from + per_state;
+            row = a.dj;
+            column = 1;
+        } else if (!STATE && a.init) {
+            from = dfrom = a.init + bh * per_state;
+        }
+        auto read = [&](f4 (&to)[NI], const float* p, int row, int column) {
+#pragma unroll
+            for (int it = 0; it < NI; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * it + 4 * lq + r, j = j0 + l16;
+                    to[it][r] = 0.0f;
+                    if (i < a.di && j < a.dj) to[it][r] = p[i * row + j * column];
+                }
+        };
+#pragma unroll
+        for (int it = 0; it < NI; ++it) c[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (from) read(c, from, row, column);
+        if constexpr (TAN) {
+#pragma unroll
+            for (int it = 0; it < NI; ++it) dc[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (from && (a.scanned || len > 0)) read(dc, dfrom, row, column);
+        }
+        if (!a.scanned && len > 0 && !a.reverse)
+#pragma unroll
+            for (int it = 0; it < NI; ++it) c[it] *= gf;
+        // few segments: what the ones before leave is added up here
+        if (!STATE && !a.scanned)
+            for (int s = 0; s < seg; ++s) {
+                const int64_t rest = len - static_cast<int64_t>(s) * a.seg_len;
+                const int64_t steps = rest < 0 ? 0 : rest < a.seg_len ? rest : a.seg_len;
+                const float w = static_cast<float>(power(g, steps));
+                f4 u[NI];
+                if constexpr (TAN) {
+                    const float dw = steps ? static_cast<float>(steps * power(g, steps - 1)) : 0.0f;
+                    read(u, slots + s * each + per_state, a.dj, 1);
+#pragma unroll
+                    for (int it = 0; it < NI; ++it) dc[it] = w * dc[it] + (dw * c[it] + u[it]);
+                }
+                read(u, slots + s * each, a.dj, 1);
+#pragma unroll
+                for (int it = 0; it < NI; ++it) c[it] = w * c[it] + u[it];
+            }
+    }
+    double slope = 0.0;
+    __syncthreads();
+    // One chunk, of which the first 16 `tiles` positions can be valid.
+    auto chunk = [&](auto tiles, int64_t pc) {
+        constexpr int kTiles = decltype(tiles)::value;
+        const int tid = form_again(threadIdx.x), lane = tid & 63, l16 = tid & 15, lq = tid >> 4 & 3;
+        const int n = positions(pc);
         // behind the sequence's last position a forward pass leaves S, not g S
-        const int m = n - (!STATE && !a.reverse && pc + n == len ? 1 : 0);
-        __syncthreads();                       // everybody is done with the rows of the last chunk
+        const int m = n - (!STATE && !a.reverse && p0 + pc + n == len ? 1 : 0);
+        // two buffers in turn: a wavefront may still read the last chunk's rows here, the ones before that nobody does
+        float* const q_s = q_all + (STATE ? 0 : (pc / kChunk & 1) * kRows);
+        float* const k_s = k_all + (pc / kChunk & 1) * kRows;
+        if (n < kChunk) {
 #pragma unroll
-        for (int x = 0; x < kLoadQ; ++x) {
-            const int e = tid + x * kBlock, at = e / kRowQ * LD + e % kRowQ * 4;
-            if (!STATE) *reinterpret_cast<f4*>(q_s + at) = q_n[x];
-            *reinterpret_cast<f4*>(k_s + at) = k_n[x];
-        }
-#pragma unroll
-        for (int x = 0; x < kLoadV; ++x) {
-            const int e = tid + x * kBlock;
-            *reinterpret_cast<f4*>(v_s + e / kRowV * LDV + e % kRowV * 4) = v_n[x];
-        }
-        __syncthreads();
-        if (pc + kChunk < pe) fetch(pc + kChunk);
-
-        // v[b][j] for b = 16 bt + 4 lq + r, j = own column: an operand of both products that use v
-        float v_r[NJ][2][4];
-#pragma unroll
-        for (int jt = 0; jt < NJ; ++jt)
+            for (int x = 0; x < kLoads; ++x)
+                if ((tid + x * kThreads) / kRowQ % kChunk >= n) {
+                    k_n[x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (!STATE) q_n[x] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
 #pragma unroll
             for (int bt = 0; bt < 2; ++bt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    v_r[jt][bt][r] = v_s[(16 * bt + 4 * lq + r) * LDV + 16 * (4 * jt + wave) + l16];
+                    if (16 * bt + 4 * lq + r >= n) v_n[bt][r] = 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < kLoads; ++x) {
+            const int e = tid + x * kThreads, at = e / kRowQ % kChunk * LD + piece_col(e);
+            if ((kPieces % kThreads && e >= kPieces) || e % kRowQ * 4 >= a.di) continue;
+            if (NARROW) {
+#pragma unroll
+                for (int r = 0; r < 3; ++r)
+                    if (r < a.di) {
+                        if (!STATE) q_s[at + r] = q_n[x][r];
+                        k_s[at + r] = k_n[x][r];
+                    }
+            } else if (a.di & 3) {             // pieces that do not begin at multiples of 16 bytes
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (!STATE) q_s[at + r] = q_n[x][r];
+                    k_s[at + r] = k_n[x][r];
+                }
+            } else {
+                if (!STATE) *reinterpret_cast<f4*>(q_s + at) = q_n[x];
+                *reinterpret_cast<f4*>(k_s + at) = k_n[x];
+            }
+        }
+        // v[b][j] for b = 16 bt + 4 lq + r, j = own column: an operand of both products that use v. Taken over here,
+        // before the next loads are under way: behind them it would wait for them too.
+        float v_r[2][4];
+#pragma unroll
+        for (int bt = 0; bt < 2; ++bt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v_r[bt][r] = v_n[bt][r];
+                asm volatile("" : "+v"(v_r[bt][r]));
+            }
+        __syncthreads();
+        q += move_i;
+        k += move_i;
+        v += move_j;
+        if (pc + kChunk < pe - p0) fetch(positions(pc + kChunk));
 
-        f4 o[NJ][2], dz[TAN ? NJ : 1][2];
+        f4 o[2], dz[2];
         if constexpr (!STATE) {
-            // scores k_b . q_a of the tiles (b, a) = (0, 0), (0, 1), (1, 1), one wavefront each
-            if (wave < 3) {
+            // scores k_b . q_a g^(a-b) of the tiles (b, a) = (0, 0), (0, 1), (1, 1), one wavefront each
+            if (wave < (kTiles == 2 ? 3 : 1)) {
                 const int bt = wave >> 1, at = (wave + 1) >> 1;
-                f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float* kp = k_s + (16 * bt + l16) * LD + 4 * lq;
+                const float* qp = q_s + (16 * at + l16) * LD + 4 * lq;
+                f4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s, kf[2], qf[2];
+                kf[0] = *reinterpret_cast<const f4*>(kp);
+                qf[0] = *reinterpret_cast<const f4*>(qp);
 #pragma unroll
                 for (int it = 0; it < NI; ++it) {
-                    if (it >= ni) break;
-                    const f4 kf = *reinterpret_cast<const f4*>(k_s + (16 * bt + l16) * LD + 16 * it + 4 * lq);
-                    const f4 qf = *reinterpret_cast<const f4*>(q_s + (16 * at + l16) * LD + 16 * it + 4 * lq);
+                    if (it + 1 < NI) {
+                        kf[(it + 1) & 1] = *reinterpret_cast<const f4*>(kp + 16 * (it + 1));
+                        qf[(it + 1) & 1] = *reinterpret_cast<const f4*>(qp + 16 * (it + 1));
+                    }
+                    one_step_ahead();
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s = mfma(kf[r], qf[r], s);
+                    for (int r = 0; r < 4; r += 2) {
+                        s = mfma(kf[it & 1][r], qf[it & 1][r], s);
+                        s2 = mfma(kf[it & 1][r + 1], qf[it & 1][r + 1], s2);
+                    }
                 }
                 f4 w, dw;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int e = 16 * (at - bt) + l16 - 4 * lq - r;
-                    const float x = a.kv_scale * s[r];
-                    w[r] = e >= 0 ? pw[e] * x : 0.0f;
-                    dw[r] = e >= 0 ? sl[e] * x : 0.0f;
+                    const int e = 16 * (at - bt) + l16 - 4 * lq - r;      // a - b; below 0: 0 whatever the score
+                    const float x = s[r] + s2[r];
+                    w[r] = e >= 0 ? x * pk[e] : 0.0f;
+                    dw[r] = e >= 0 ? x * sk[e] : 0.0f;
                 }
                 score_s[wave * kWave + lane] = w;
                 if (TAN) score_s[(3 + wave) * kWave + lane] = dw;
             }
             // q C
+            if (mine) {
 #pragma unroll
-            for (int at = 0; at < 2; ++at) {
+                for (int at = 0; at < 2; ++at) o[at] = dz[at] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                {
+                    f4 qf[2][2];
+                    auto read = [&](int it) {
 #pragma unroll
-                for (int jt = 0; jt < NJ; ++jt) {
-                    o[jt][at] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (TAN) dz[jt][at] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int at = 0; at < kTiles; ++at)
+                            qf[it & 1][at] = *reinterpret_cast<const f4*>(q_s + (16 * at + l16) * LD + 16 * it + 4 * lq);
+                    };
+                    read(0);
+#pragma unroll
+                    for (int it = 0; it < NI; ++it) {
+                        if (it + 1 < NI) read(it + 1);
+                        one_step_ahead();
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int at = 0; at < kTiles; ++at) {
+                                o[at] = mfma(c[it][r], qf[it & 1][at][r], o[at]);
+                                if (TAN) dz[at] = mfma(dc[it][r], qf[it & 1][at][r], dz[at]);
+                            }
+                    }
                 }
 #pragma unroll
-                for (int it = 0; it < NI; ++it) {
-                    if (it >= ni) break;
-                    const f4 qf = *reinterpret_cast<const f4*>(q_s + (16 * at + l16) * LD + 16 * it + 4 * lq);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int jt = 0; jt < NJ; ++jt) {
-                            o[jt][at] = mfma(c[it][jt][r], qf[r], o[jt][at]);
-                            if (TAN) dz[jt][at] = mfma(dc[it][jt][r], qf[r], dz[jt][at]);
-                        }
-                }
-            }
-#pragma unroll
-            for (int at = 0; at < 2; ++at) {
-                const float w = pw[16 * at + l16], dw = sl[16 * at + l16];
-#pragma unroll
-                for (int jt = 0; jt < NJ; ++jt) {
-                    if (TAN) dz[jt][at] = w * dz[jt][at] + dw * o[jt][at];
-                    o[jt][at] = w * o[jt][at];
+                for (int at = 0; at < 2; ++at) {
+                    const float w = pw[16 * at + l16], dw = sl[16 * at + l16];
+                    if (TAN) dz[at] = w * dz[at] + dw * o[at];
+                    o[at] = w * o[at];
                 }
             }
         }
         // C = g^m C + sum_b g^(m-b) k_b^T v_b
-        {
-            float vw[NJ][2][4], vs[TAN ? NJ : 1][2][4];
+        if (mine) {
+            float vw[2][4], vs[2][4];
 #pragma unroll
             for (int bt = 0; bt < 2; ++bt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int e = m - (16 * bt + 4 * lq + r);       // below 0 only where v is 0
-                    const float w = a.kv_scale * pw[e > 0 ? e : 0], dw = a.kv_scale * sl[e > 0 ? e : 0];
+                    vw[bt][r] = pk[e > 0 ? e : 0] * v_r[bt][r];
+                    if (TAN) vs[bt][r] = sk[e > 0 ? e : 0] * v_r[bt][r];
+                }
+            const float w = pw[m], wl = pl[m], dw = sl[m];
+            {
+                float kf[2][8];
+                auto read = [&](int it) {
 #pragma unroll
-                    for (int jt = 0; jt < NJ; ++jt) {
-                        vw[jt][bt][r] = w * v_r[jt][bt][r];
-                        if (TAN) vs[jt][bt][r] = dw * v_r[jt][bt][r];
+                    for (int x = 0; x < 4 * kTiles; ++x)
+                        kf[it & 1][x] = k_s[(16 * (x >> 2) + 4 * lq + (x & 3)) * LD + 16 * it + l16];
+                };
+                read(0);
+#pragma unroll
+                for (int it = 0; it < NI; ++it) {
+                    if (it + 1 < NI) read(it + 1);
+                    one_step_ahead();
+                    // the power with what its rounding left: the same factor every 32 positions
+                    if (TAN) dc[it] = w * dc[it] + (wl * dc[it] + dw * c[it]);
+                    c[it] = w * c[it] + wl * c[it];
+#pragma unroll
+                    for (int x = 0; x < 4 * kTiles; ++x) {
+                        c[it] = mfma(kf[it & 1][x], vw[x >> 2][x & 3], c[it]);
+                        if (TAN) dc[it] = mfma(kf[it & 1][x], vs[x >> 2][x & 3], dc[it]);
                     }
                 }
-            const float w = pw[m], dw = sl[m];
-#pragma unroll
-            for (int it = 0; it < NI; ++it) {
-                if (it >= ni) break;
-#pragma unroll
-                for (int jt = 0; jt < NJ; ++jt) {
-                    if (TAN) dc[it][jt] = w * dc[it][jt] + dw * c[it][jt];
-                    c[it][jt] = w * c[it][jt];
-                }
-#pragma unroll
-                for (int bt = 0; bt < 2; ++bt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float kf = k_s[(16 * bt + 4 * lq + r) * LD + 16 * it + l16];
-#pragma unroll
-                        for (int jt = 0; jt < NJ; ++jt) {
-                            c[it][jt] = mfma(kf, vw[jt][bt][r], c[it][jt]);
-                            if (TAN) dc[it][jt] = mfma(kf, vs[jt][bt][r], dc[it][jt]);
-                        }
-                    }
             }
         }
         if constexpr (!STATE) {
             __syncthreads();                   // the scores are there
+            if (!mine) return;
             // A product with a score of 0 would carry a NaN or an infinity of v to positions before it: such values
             // are left out of the products and added to their own and later positions one by one.
-            bool finite = true;
+            float nothing = 0.0f;                      // a NaN if one of the values is not finite
 #pragma unroll
-            for (int jt = 0; jt < NJ; ++jt)
+            for (int bt = 0; bt < kTiles; ++bt)
 #pragma unroll
-                for (int bt = 0; bt < 2; ++bt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) finite = finite && __builtin_isfinite(v_r[jt][bt][r]);
-            const bool all_finite = __all(finite);
+                for (int r = 0; r < 4; ++r) nothing += 0.0f * v_r[bt][r];
+            const bool all_finite = __all(nothing == 0.0f);
             if (!all_finite)
 #pragma unroll
-                for (int jt = 0; jt < NJ; ++jt)
+                for (int bt = 0; bt < kTiles; ++bt)
 #pragma unroll
-                    for (int bt = 0; bt < 2; ++bt)
+                    for (int r = 0; r < 4; ++r) v_r[bt][r] = __builtin_isfinite(v_r[bt][r]) ? v_r[bt][r] : 0.0f;
+            f4 w[3], dw[3];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!__builtin_isfinite(v_r[jt][bt][r])) v_r[jt][bt][r] = 0.0f;
+            for (int tile = 0; tile < (kTiles == 2 ? 3 : 1); ++tile) {
+                w[tile] = score_s[tile * kWave + lane];
+                if (TAN) dw[tile] = score_s[(3 + tile) * kWave + lane];
+            }
 #pragma unroll
-            for (int at = 0; at < 2; ++at)
+            for (int bt = 0; bt < kTiles; ++bt)
 #pragma unroll
-                for (int bt = 0; bt <= at; ++bt) {
-                    const f4 w = score_s[(bt + at) * kWave + lane];
-                    f4 dw;
-                    if (TAN) dw = score_s[(3 + bt + at) * kWave + lane];
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int at = bt; at < kTiles; ++at) {
+                        o[at] = mfma(v_r[bt][r], w[bt + at][r], o[at]);
+                        if (TAN) dz[at] = mfma(v_r[bt][r], dw[bt + at][r], dz[at]);
+                    }
+            const int left = a.dj - j0 - 4 * lq;
+            if (!all_finite) {
+                const float* here = v - move_j;
+                const float* score = reinterpret_cast<const float*>(score_s);
+                for (int x = 0; x < n; ++x) {
+                    const f4 vx = load4(at_offset(here, row_offset(x, step_j32) + 16 * lq), left);
+#pragma unroll
+                    for (int at = 0; at < kTiles; ++at) {
+                        if (16 * at + l16 < x) continue;
+                        const int from = (((x >> 4) + at) * kWave + (x >> 2 & 3) * 16 + l16) * 4 + (x & 3);
+                        const float wx = score[from], dwx = TAN ? score[from + 12 * kWave] : 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (__builtin_isfinite(vx[r])) continue;
+                            o[at][r] += wx * vx[r];
+                            if (TAN) dz[at][r] += dwx * vx[r];
+                        }
+                    }
+                }
+            }
+            // lane: position 16 at + l16, columns j0 + 4 lq .. + 3
+#pragma unroll
+            for (int at = 0; at < kTiles; ++at) {
+                if (16 * at + l16 >= n) continue;
+                const uint32_t row = row_offset(16 * at + l16, step_j32) + 16 * lq;
+                store4(const_cast<float*>(at_offset(out, row)), a.out_scale * o[at], left);
+                if (TAN) {
+                    const f4 zx = load4(at_offset(z, row), left);
+                    float s = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int jt = 0; jt < NJ; ++jt) {
-                            o[jt][at] = mfma(v_r[jt][bt][r], w[r], o[jt][at]);
-                            if (TAN) dz[jt][at] = mfma(v_r[jt][bt][r], dw[r], dz[jt][at]);
-                        }
-                }
-            if (!all_finite) {
-                const float* score = reinterpret_cast<const float*>(score_s);
-#pragma unroll
-                for (int at = 0; at < 2; ++at)
-                    for (int x = 0; x <= 16 * at + l16; ++x) {
-                        const int e = (((x >> 4) + at) * kWave + (x >> 2 & 3) * 16 + l16) * 4 + (x & 3);
-                        const float w = score[e], dw = TAN ? score[e + 12 * kWave] : 0.0f;
-#pragma unroll
-                        for (int jt = 0; jt < NJ; ++jt) {
-                            const f4 vx = *reinterpret_cast<const f4*>(v_s + x * LDV + 16 * (4 * jt + wave) + 4 * lq);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                if (__builtin_isfinite(vx[r])) continue;
-                                o[jt][at][r] += w * vx[r];
-                                if (TAN) dz[jt][at][r] += dw * vx[r];
-                            }
-                        }
-                    }
-            }
-            // lane: position 16 at + l16, columns 16 (4 jt + wave) + 4 lq .. + 3
-#pragma unroll
-            for (int at = 0; at < 2; ++at) {
-                if (16 * at + l16 >= n) continue;
-                const int64_t row = time_of(pc + 16 * at + l16) * step_j + bh * a.dj + jt0;
-#pragma unroll
-                for (int jt = 0; jt < NJ; ++jt) {
-                    const int j = 16 * (4 * jt + wave) + 4 * lq;
-                    if (j >= dj) continue;
-                    store4(a.out + row + j, a.out_scale * o[jt][at], dj - j);
-                    if (TAN) {
-                        const f4 z = load4(a.z + row + j, dj - j);
-                        float s = 0.0f;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) s += z[r] * dz[jt][at][r];
-                        slope += static_cast<double>(a.out_scale * s);
-                    }
+                        if (r < left) s += zx[r] * dz[at][r];
+                    slope += static_cast<double>(a.out_scale * s);
                 }
             }
         }
-    }
+    };
+    int64_t pc = 0;
+    for (; pe - p0 - pc > 16; pc += kChunk, out += move_j, z += TAN ? move_j : 0) chunk(std::integral_constant<int, 2>{}, pc);
+    for (; pc < pe - p0; pc += 16) chunk(std::integral_constant<int, 1>{}, pc);
 
     if constexpr (STATE) {
 #pragma unroll
         for (int it = 0; it < NI; ++it)
 #pragma unroll
-            for (int jt = 0; jt < NJ; ++jt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * lq + r, j = 16 * (4 * jt + wave) + l16;
-                    if (i >= a.di || j >= dj) continue;
-                    float* s = a.seg + (bh * a.segs + seg) * per_state * (TAN ? 2 : 1) + static_cast<int64_t>(i) * a.dj +
-                               jt0 + j;
-                    s[0] = c[it][jt][r];
-                    if (TAN) s[per_state] = dc[it][jt][r];
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * it + 4 * lq + r, j = j0 + l16;
+                if (i >= a.di || j >= a.dj) continue;
+                float* s = a.seg + (bh * a.segs + seg) * per_state * (TAN ? 2 : 1) + i * a.dj + j;
+                s[0] = c[it][r];
+                if (TAN) s[per_state] = dc[it][r];
+            }
         return;
     }
-    // rows behind the sequence's end
-    {
-        const int64_t first = len > p0 ? len : p0;
-        const int width = dj < 64 * NJ ? dj : 64 * NJ;
-        for (int64_t p = first + wave; p < p1; p += 4)
-            for (int j = lane; j < width; j += kWave) a.out[p * step_j + bh * a.dj + jt0 + j] = 0.0f;
-    }
+    // rows behind the sequence's end: there position p is time p in both directions
+    for (int64_t p = (len > p0 ? len : p0) + wave; p < p1; p += NW)
+        for (int j = lane; j < a.dj; j += kWave) a.out[(p * a.batch * a.heads + bh) * a.dj + j] = 0.0f;
     // the workgroup of the segment with the last position has the final state
     const bool last = len > 0 ? (pe == len && pe > p0) : seg == 0;
     if (last && (a.fin || (TAN && a.dfin))) {
 #pragma unroll
         for (int it = 0; it < NI; ++it)
 #pragma unroll
-            for (int jt = 0; jt < NJ; ++jt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * lq + r, j = 16 * (4 * jt + wave) + l16;
-                    if (i >= a.di || j >= dj) continue;
-                    const int64_t at = bh * per_state + static_cast<int64_t>(i) * a.si + static_cast<int64_t>(jt0 + j) * a.sj;
-                    if (a.fin) a.fin[at] = c[it][jt][r];
-                    if (TAN && a.dfin) slope += static_cast<double>(a.dfin[at]) * dc[it][jt][r];
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * it + 4 * lq + r, j = j0 + l16;
+                if (i >= a.di || j >= a.dj) continue;
+                const int64_t at = bh * per_state + i * a.si + j * a.sj;
+                if (a.fin) a.fin[at] = c[it][r];
+                if (TAN && a.dfin) slope += static_cast<double>(a.dfin[at]) * dc[it][r];
+            }
     }
     if constexpr (TAN) {
         for (int d = 1; d < kWave; d <<= 1) slope += __shfl_xor(slope, d);
         if (lane == 0) part_s[wave] = slope;
         __syncthreads();
-        if (tid == 0) a.slope[blockIdx.x] = (part_s[0] + part_s[1]) + (part_s[2] + part_s[3]);
+        if (tid == 0) {
+            double s = 0.0;
+            for (int x = 0; x < NW; ++x) s += part_s[x];
+            a.slope[blockIdx.x] = s;
+        }
     }
 }
 
-// Turns the states that the segments leave when they start from zero into the states they start from.
-__global__ __launch_bounds__(kBlock) void la_scan_kernel(PassArgs a, int tangent) {
+// Short sequences without a state before or behind them: all scores are formed, none goes through a state. With d
+// features a position costs 4 d (T / 2) operations instead of the 4 d^2 + 128 d of a pass in chunks.
+//
+// A wavefront has the 16 positions of one tile: q as operands in registers, the sums over v as accumulators. The
+// rows of k and v come through LDS in steps of 32 positions; a tile of scores (b, a) is at once the operand of its
+// product with v. Tile n has n + 1 tiles of scores: wavefronts s and s + 4, which share a SIMD, take tiles whose work adds
+// up to the same.
+constexpr int kAllScores = 128;        // positions that eight wavefronts cover
+template <int NI, int NJ, bool TAN>
+__global__ __launch_bounds__(8 * kWave, TAN ? 2 : 4) void la_scores_kernel(Passes passes) {
+    constexpr int LD = 16 * NI + 4, LDV = 16 * NJ + 4, kThreads = 8 * kWave;
+    constexpr int kRowsK = kChunk * LD, kRowsV = kChunk * LDV;
+    __shared__ __attribute__((aligned(16))) float k_all[2 * kRowsK], v_all[2 * kRowsV];
+    __shared__ float pk[kAllScores], sk[TAN ? kAllScores : 1];       // kv_scale times g^n and n g^(n-1)
+    __shared__ double part_s[8];
+
+    const PassArgs& a = passes.pass[blockIdx.y];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, lq = lane >> 4;
+    const int64_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
+    const int len = static_cast<int>(sequence_length(a.lengths, b, a.time));
+    const int tiles = (len + 15) >> 4;
+    const int mine = wave < 4 ? tiles - 1 - wave : wave - 4 - (8 - tiles);       // the tile of this wavefront, or < 0
+    const int p = mine >= 0 ? 16 * mine + l16 : 0;                               // this lane's position as a column
+    // position p is time p forwards, len - 1 - p backwards
+    const int64_t step_i = a.batch * a.heads * a.di, step_j = a.batch * a.heads * a.dj;
+    auto time_of = [&](int x) { return a.reverse ? len - 1 - x : x; };
+
+    // ---- rows of the next 32 positions, on their way from memory; rows behind the last are taken from the last
+    constexpr int kPiecesK = kChunk * 4 * NI, kPiecesV = kChunk * 4 * NJ;
+    constexpr int kLoadsK = (kPiecesK + kThreads - 1) / kThreads, kLoadsV = (kPiecesV + kThreads - 1) / kThreads;
+    auto piece_col = [](int e, int per_row, int d) {
+        const int col = e % per_row * 4;
+        return col >= d ? 0 : col + 4 > d ? d - 4 : col;
+    };
+    f4 k_n[kLoadsK], v_n[kLoadsV];
+    auto fetch = [&](int first) {
+        const int tid = form_again(threadIdx.x);
+#pragma unroll
+        for (int m = 0; m < kLoadsK; ++m) {
+            const int e = tid + m * kThreads, x = first + e / (4 * NI) % kChunk;
+            k_n[m] = *reinterpret_cast<const f4u*>(a.k + time_of(x < len ? x : len - 1) * step_i + bh * a.di + piece_col(e, 4 * NI, a.di));
+        }
+#pragma unroll
+        for (int m = 0; m < kLoadsV; ++m) {
+            const int e = tid + m * kThreads, x = first + e / (4 * NJ) % kChunk;
+            v_n[m] = *reinterpret_cast<const f4u*>(a.v + time_of(x < len ? x : len - 1) * step_j + bh * a.dj + piece_col(e, 4 * NJ, a.dj));
+        }
+    };
+    auto put = [&](float* to, const f4& x, int e, int pieces, int per_row, int d, int ld) {
+        if (e >= pieces || e % per_row * 4 >= d) return;
+        float* at = to + e / per_row * ld + piece_col(e, per_row, d);
+        if (d & 3) {                           // pieces that do not begin at multiples of 16 bytes
+#pragma unroll
+            for (int r = 0; r < 4; ++r) at[r] = x[r];
+        } else {
+            *reinterpret_cast<f4*>(at) = x;
+        }
+    };
+    f4 qf[NI];
+    if (len > 0) {
+        fetch(0);
+        const float* q = a.q + time_of(p < len ? p : len - 1) * step_i + bh * a.di;
+#pragma unroll
+        for (int it = 0; it < NI; ++it) {
+            const int col = 16 * it + 4 * lq;
+            qf[it] = *reinterpret_cast<const f4u*>(q + (col + 4 <= a.di ? col : a.di - 4));
+        }
+        // the piece with the row's end was read up to it; what is behind the end is 0
+#pragma unroll
+        for (int it = 0; it < NI; ++it) {
+            const int over = 16 * it + 4 * lq + 4 - a.di;
+            f4 x = qf[it];
+            if (over == 1) x = f4{x[1], x[2], x[3], 0.0f};
+            if (over == 2) x = f4{x[2], x[3], 0.0f, 0.0f};
+            if (over == 3) x = f4{x[3], 0.0f, 0.0f, 0.0f};
+            if (over > 3) x = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            qf[it] = x;
+        }
+    }
+    if (tid < kAllScores) {
+        const double g = a.decay[h];
+        pk[tid] = a.kv_scale * static_cast<float>(power(g, tid));
+        if (TAN) sk[tid] = tid ? a.kv_scale * static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
+    }
+    // columns that a row does not have: zeros, which nothing overwrites
+    for (int e = tid * 4; e < 2 * kRowsK; e += kThreads * 4) *reinterpret_cast<f4*>(k_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e = tid * 4; e < 2 * kRowsV; e += kThreads * 4) *reinterpret_cast<f4*>(v_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    f4 o[NJ], dz[TAN ? NJ : 1];
+#pragma unroll
+    for (int jt = 0; jt < NJ; ++jt) {
+        o[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (TAN) dz[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __syncthreads();
+
+    for (int first = 0; first < len; first += kChunk) {
+        float* const k_s = k_all + (first / kChunk & 1) * kRowsK;
+        float* const v_s = v_all + (first / kChunk & 1) * kRowsV;
+#pragma unroll
+        for (int m = 0; m < kLoadsK; ++m) put(k_s, k_n[m], tid + m * kThreads, kPiecesK, 4 * NI, a.di, LD);
+#pragma unroll
+        for (int m = 0; m < kLoadsV; ++m) put(v_s, v_n[m], tid + m * kThreads, kPiecesV, 4 * NJ, a.dj, LDV);
+        __syncthreads();                       // two buffers: nobody reads the ones before the last any more
+        if (first + kChunk < len) fetch(first + kChunk);
+        for (int x = first; x < first + kChunk && x <= 16 * mine; x += 16) {
+            const float* kp = k_s + (x - first + l16) * LD + 4 * lq;
+            const float* vp = v_s + (x - first + 4 * lq) * LDV + l16;
+            f4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s, kf[2];
+            kf[0] = *reinterpret_cast<const f4*>(kp);
+#pragma unroll
+            for (int it = 0; it < NI; ++it) {
+                if (it + 1 < NI) kf[(it + 1) & 1] = *reinterpret_cast<const f4*>(kp + 16 * (it + 1));
+                one_step_ahead();
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    s = mfma(kf[it & 1][r], qf[it][r], s);
+                    s2 = mfma(kf[it & 1][r + 1], qf[it][r + 1], s2);
+                }
+            }
+            const int distance = 16 * mine + l16 - x - 4 * lq;           // a - b of r = 0
+            float w[4], dw[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int e = distance - r;                              // below 0: 0 whatever the score
+                const float y = s[r] + s2[r];
+                w[r] = e >= 0 ? y * pk[e] : 0.0f;
+                dw[r] = TAN && e >= 0 ? y * sk[e] : 0.0f;
+            }
+            float vf[2][4];
+            auto read = [&](int jt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vf[jt & 1][r] = vp[r * LDV + 16 * jt];
+            };
+            read(0);
+            float nothing = 0.0f;                                        // a NaN if a value of v is not finite
+#pragma unroll
+            for (int jt = 0; jt < NJ; ++jt) {
+                if (jt + 1 < NJ) read(jt + 1);
+                one_step_ahead();
+                // on the diagonal a score of 0 would carry a NaN or an infinity to positions before it
+                if (x == 16 * mine)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        nothing += 0.0f * vf[jt & 1][r];
+                        vf[jt & 1][r] = __builtin_isfinite(vf[jt & 1][r]) ? vf[jt & 1][r] : 0.0f;
+                    }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    o[jt] = mfma(vf[jt & 1][r], w[r], o[jt]);
+                    if (TAN) dz[jt] = mfma(vf[jt & 1][r], dw[r], dz[jt]);
+                }
+            }
+            if (!__all(nothing == 0.0f)) {                               // such values reach their own and later positions
+                for (int y = 0; y < 16; ++y) {
+                    // the score of b = y, a = this lane's: lane 16 (y / 4) + l16, element y % 4
+                    const int from = 16 * (y >> 2) + l16;
+                    float wy = 0.0f, dwy = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w0 = __shfl(w[r], from), w1 = __shfl(dw[r], from);
+                        if ((y & 3) == r) {
+                            wy = w0;
+                            dwy = w1;
+                        }
+                    }
+                    if (l16 < y) continue;
+#pragma unroll
+                    for (int jt = 0; jt < NJ; ++jt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float vy = v_s[(x - first + y) * LDV + 16 * jt + 4 * lq + r];
+                            if (__builtin_isfinite(vy)) continue;
+                            o[jt][r] += wy * vy;
+                            if (TAN) dz[jt][r] += dwy * vy;
+                        }
+                }
+            }
+        }
+    }
+
+    // lane: position p, columns 16 jt + 4 lq .. + 3
+    double slope = 0.0;
+    if (mine >= 0 && p < len) {
+        const int64_t row = time_of(p) * step_j + bh * a.dj;
+#pragma unroll
+        for (int jt = 0; jt < NJ; ++jt) {
+            const int col = 16 * jt + 4 * lq, left = a.dj - col;
+            if (left <= 0) continue;
+            store4(a.out + row + col, a.out_scale * o[jt], left);
+            if (TAN) {
+                const f4 z = load4(a.z + row + col, left);
+                float s = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < left) s += z[r] * dz[jt][r];
+                slope += static_cast<double>(a.out_scale * s);
+            }
+        }
+    }
+    // rows behind the sequence's end
+    for (int64_t x = len + wave; x < a.time; x += 8)
+        for (int j = lane; j < a.dj; j += kWave) a.out[x * step_j + bh * a.dj + j] = 0.0f;
+    if constexpr (TAN) {
+        for (int d = 1; d < kWave; d <<= 1) slope += __shfl_xor(slope, d);
+        if (lane == 0) part_s[wave] = slope;
+        __syncthreads();
+        if (tid == 0) {
+            double s = 0.0;
+            for (int x = 0; x < 8; ++x) s += part_s[x];
+            a.slope[blockIdx.x] = s;
+        }
+    }
+}
+
+constexpr int kScanned = 32;
+// Turns the states that the segments leave when they start from zero into the states they start from; the loads of
+// kScanned segments at a time do not wait for each other.
+__global__ __launch_bounds__(kBlock) void la_scan_kernel(Passes passes, int tangent) {
+    const PassArgs& a = passes.pass[blockIdx.z];
     const int64_t per_state = static_cast<int64_t>(a.di) * a.dj;
     const int64_t e = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-    const int64_t bh = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 65535;
-    if (e >= per_state || bh >= a.batch * a.heads) return;
-    const int64_t len = sequence_length(a.lengths, bh / a.heads, a.time);
-    const double g = a.decay[bh % a.heads];
-    const float full = static_cast<float>(power(g, a.seg_len));
-    const float dfull = static_cast<float>(a.seg_len * power(g, a.seg_len - 1));
-    float c = 0.0f, dc = 0.0f;
-    if (a.init) {
-        const float s = a.init[bh * per_state + e / a.dj * a.si + e % a.dj * a.sj];
-        c = len > 0 && !a.reverse ? static_cast<float>(g) * s : s;
-        dc = len > 0 ? s : 0.0f;
-    }
-    float* slot = a.seg + bh * a.segs * per_state * (1 + tangent) + e;
-    for (int seg = 0; seg < a.segs; ++seg, slot += per_state * (1 + tangent)) {
-        const bool more = seg + 1 < a.segs;
-        const float u = more ? slot[0] : 0.0f;
-        const float du = more && tangent ? slot[per_state] : 0.0f;
-        slot[0] = c;
-        if (tangent) slot[per_state] = dc;
-        const int64_t left = len - static_cast<int64_t>(seg) * a.seg_len;
-        float w = full, dw = dfull;
-        if (left < a.seg_len) {
-            w = static_cast<float>(power(g, left > 0 ? left : 0));
-            dw = left > 0 ? static_cast<float>(left * power(g, left - 1)) : 0.0f;
+    if (e >= per_state) return;
+    for (int64_t bh = blockIdx.y; bh < a.batch * a.heads; bh += gridDim.y) {
+        const int64_t len = sequence_length(a.lengths, bh / a.heads, a.time);
+        const double g = a.decay[bh % a.heads];
+        const double full = power(g, a.seg_len), dfull = a.seg_len * power(g, a.seg_len - 1);
+        double c = 0.0, dc = 0.0;
+        if (a.init) {
+            const float s = a.init[bh * per_state + e / a.dj * a.si + e % a.dj * a.sj];
+            c = len > 0 && !a.reverse ? static_cast<float>(g) * s : s;
+            dc = len > 0 ? s : 0.0f;
         }
-        dc = w * dc + dw * c + du;
-        c = w * c + u;
+        const int64_t step = per_state * (1 + tangent);
+        float* slot = a.seg + bh * a.segs * step + e;
+        for (int first = 0; first < a.segs; first += kScanned, slot += kScanned * step) {
+            float u[kScanned], du[kScanned];
+#pragma unroll
+            for (int x = 0; x < kScanned; ++x) {
+                const bool more = first + x + 1 < a.segs;            // the last segment's was not formed
+                u[x] = more ? slot[x * step] : 0.0f;
+                du[x] = more && tangent ? slot[x * step + per_state] : 0.0f;
+            }
+#pragma unroll
+            for (int x = 0; x < kScanned; ++x) {
+                if (first + x >= a.segs) break;
+                slot[x * step] = static_cast<float>(c);
+                if (tangent) slot[x * step + per_state] = static_cast<float>(dc);
+                const int64_t left = len - static_cast<int64_t>(first + x) * a.seg_len;
+                double w = full, dw = dfull;
+                if (left < a.seg_len) {
+                    w = power(g, left > 0 ? left : 0);
+                    dw = left > 0 ? left * power(g, left - 1) : 0.0;
+                }
+                dc = w * dc + dw * c + du[x];
+                c = w * c + u[x];
+            }
+        }
     }
 }
 
@@ -549,70 +920,116 @@ struct Scratch {
     int get(size_t n) { return pool_alloc_raw(n, &p); }
 };
 
-template <int NI, bool TAN, bool STATE>
-void launch_pass(const PassArgs& a, int nj, unsigned grid) {
-    if (nj == 1)
-        hipLaunchKernelGGL((la_pass_kernel<NI, 1, TAN, STATE>), dim3(grid), dim3(kBlock), 0, ctx().stream, a);
-    else
-        hipLaunchKernelGGL((la_pass_kernel<NI, 2, TAN, STATE>), dim3(grid), dim3(kBlock), 0, ctx().stream, a);
+template <int NI, bool TAN, bool STATE, bool NARROW = false>
+void launch_pass(const Passes& p, int dj, dim3 grid) {
+    if (dj <= 64) hipLaunchKernelGGL((la_pass_kernel<NI, 4, TAN, STATE, NARROW>), grid, dim3(4 * kWave), 0, ctx().stream, p);
+    else hipLaunchKernelGGL((la_pass_kernel<NI, 8, TAN, STATE, NARROW>), grid, dim3(8 * kWave), 0, ctx().stream, p);
 }
 template <bool TAN, bool STATE>
-void launch_pass(const PassArgs& a, int nj, unsigned grid) {
-    if (a.di <= 32) launch_pass<2, TAN, STATE>(a, nj, grid);
-    else if (a.di <= 64) launch_pass<4, TAN, STATE>(a, nj, grid);
-    else launch_pass<8, TAN, STATE>(a, nj, grid);
+void launch_pass(const Passes& p, int di, int dj, dim3 grid) {
+    if (di < 4) launch_pass<2, TAN, STATE, true>(p, dj, grid);       // all passes of the launch, or none (bwd)
+    else if (di <= 32) launch_pass<2, TAN, STATE>(p, dj, grid);
+    else if (di <= 64) launch_pass<4, TAN, STATE>(p, dj, grid);
+    else if (di <= 96) launch_pass<6, TAN, STATE>(p, dj, grid);
+    else launch_pass<8, TAN, STATE>(p, dj, grid);
 }
 
-// One pass. ddecay: with the derivative by the decay.
-int run_pass(PassArgs a, float* ddecay) {
+template <int NI, bool TAN>
+void launch_scores(const Passes& p, int dj, dim3 grid) {
+    if (dj <= 32) hipLaunchKernelGGL((la_scores_kernel<NI, 2, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
+    else if (dj <= 64) hipLaunchKernelGGL((la_scores_kernel<NI, 4, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
+    else hipLaunchKernelGGL((la_scores_kernel<NI, 8, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
+}
+template <bool TAN>
+void launch_scores(const Passes& p, int di, int dj, dim3 grid) {
+    if (di <= 32) launch_scores<2, TAN>(p, dj, grid);
+    else if (di <= 64) launch_scores<4, TAN>(p, dj, grid);
+    else launch_scores<8, TAN>(p, dj, grid);
+}
+
+// `count` passes over the same sequences side by side. ddecay: with the derivative by the decay (one pass).
+int run_passes(Passes p, int count, float* ddecay) {
+    const PassArgs& a = p.pass[0];
     const int64_t sequences = a.batch * a.heads;
-    const int64_t want = 2 * static_cast<int64_t>(ctx().num_cus);
-    const int nj = a.dj > 64 ? 2 : 1;
-    a.tiles_j = static_cast<int>(ceil_div(a.dj, 64 * nj));
-    // enough workgroups for the device: the time axis is cut, into segments of 128 positions at least
-    int64_t segs = ceil_div(want, sequences * a.tiles_j);
+    if (sequences * (a.di > a.dj ? a.di : a.dj) > kStepFloats)
+        return set_error(BSHIP_ERR_UNSUPPORTED, "linear attention: more than %lld features in a time step",
+                         static_cast<long long>(kStepFloats));
+    int di = 0, dj = 0;
+    for (int n = 0; n < count; ++n) {
+        di = p.pass[n].di > di ? p.pass[n].di : di;
+        dj = p.pass[n].dj > dj ? p.pass[n].dj : dj;
+    }
+    // all scores where that is the less work, or nearly: 2 T d against 4 d^2 and the scores inside chunks
+    bool whole = a.time <= kAllScores && a.time * (a.di + a.dj) <= 4 * a.di * a.dj + 32 * (a.di + a.dj);
+    for (int n = 0; n < count; ++n)
+        whole = whole && !p.pass[n].init && !p.pass[n].fin && !p.pass[n].dfin && p.pass[n].di >= 4 && p.pass[n].dj >= 4;
+    if (whole) {
+        Scratch slope;
+        if (ddecay) {
+            int st = slope.get(sequences * sizeof(double));
+            if (st != 0) return st;
+            p.pass[0].slope = static_cast<double*>(slope.p);
+        }
+        const dim3 grid(static_cast<unsigned>(sequences), static_cast<unsigned>(count));
+        if (ddecay) launch_scores<true>(p, di, dj, grid);
+        else launch_scores<false>(p, di, dj, grid);
+        int st = check_launch("linear attention, all scores");
+        if (st != 0 || !ddecay) return st;
+        hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(a.heads)), dim3(kBlock), 0, ctx().stream,
+                           static_cast<const double*>(slope.p), ddecay, a.batch, a.heads, int64_t(1));
+        return check_launch("linear attention, decay gradient");
+    }
+    // eight wavefronts for every compute unit: where there are fewer sequences, the time axis is cut, into segments of
+    // 128 positions at least
+    int64_t want = 8 * static_cast<int64_t>(ctx().num_cus) / (dj <= 64 ? 4 : 8);
+    int64_t segs = ceil_div(want, sequences * count);
     const int64_t most = ceil_div(a.time, 4 * kChunk);
     if (segs > most) segs = most;
     if (segs < 1) segs = 1;
     int64_t seg_len = ceil_div(ceil_div(a.time, segs), kChunk) * kChunk;
     if (seg_len < kChunk) seg_len = kChunk;
     segs = a.time > 0 ? ceil_div(a.time, seg_len) : 1;
-    if (seg_len > 0x7fffffff || sequences * segs * a.tiles_j > 0x7fffffff)
+    if (sequences * segs > 0x7fffffff)
         return set_error(BSHIP_ERR_BAD_DIMENSION, "linear attention: %lld sequences of %lld steps exceed one launch",
                          static_cast<long long>(sequences), static_cast<long long>(a.time));
-    a.segs = static_cast<int>(segs);
-    a.seg_len = static_cast<int>(seg_len);
-    const unsigned grid = static_cast<unsigned>(sequences * segs * a.tiles_j);
-    const size_t per_state = static_cast<size_t>(a.di) * a.dj;
+    const size_t states = static_cast<size_t>(sequences) * segs * a.di * a.dj * (ddecay ? 2 : 1);
     Scratch seg, slope;
     if (segs > 1) {
-        int st = seg.get(sequences * segs * per_state * (ddecay ? 2 : 1) * sizeof(float));
+        int st = seg.get(states * count * sizeof(float));
         if (st != 0) return st;
-        a.seg = static_cast<float*>(seg.p);
     }
     if (ddecay) {
-        int st = slope.get(grid * sizeof(double));
+        int st = slope.get(sequences * segs * sizeof(double));
         if (st != 0) return st;
-        a.slope = static_cast<double*>(slope.p);
     }
+    for (int n = 0; n < count; ++n) {
+        p.pass[n].segs = static_cast<int>(segs);
+        p.pass[n].seg_len = static_cast<int>(seg_len);
+        p.pass[n].scanned = segs > kAddedUp;
+        p.pass[n].seg = segs > 1 ? static_cast<float*>(seg.p) + n * states : nullptr;
+        p.pass[n].slope = static_cast<double*>(slope.p);
+    }
+    const dim3 grid(static_cast<unsigned>(sequences * segs), static_cast<unsigned>(count));
     if (segs > 1) {
-        if (ddecay) launch_pass<true, true>(a, nj, grid);
-        else launch_pass<false, true>(a, nj, grid);
+        if (ddecay) launch_pass<true, true>(p, di, dj, grid);
+        else launch_pass<false, true>(p, di, dj, grid);
         int st = check_launch("linear attention, segment states");
         if (st != 0) return st;
-        const unsigned y = static_cast<unsigned>(sequences < 65535 ? sequences : 65535);
-        hipLaunchKernelGGL(la_scan_kernel, dim3(static_cast<unsigned>(ceil_div(per_state, kBlock)), y,
-                                                static_cast<unsigned>(ceil_div(sequences, 65535))),
-                           dim3(kBlock), 0, ctx().stream, a, ddecay ? 1 : 0);
-        st = check_launch("linear attention, scan");
+    }
+    if (segs > kAddedUp) {
+        const int64_t rows = sequences < 32768 ? sequences : 32768;
+        hipLaunchKernelGGL(la_scan_kernel, dim3(static_cast<unsigned>(ceil_div(a.di * a.dj, kBlock)),
+                                                static_cast<unsigned>(rows), static_cast<unsigned>(count)),
+                           dim3(kBlock), 0, ctx().stream, p, ddecay ? 1 : 0);
+        int st = check_launch("linear attention, scan");
         if (st != 0) return st;
     }
-    if (ddecay) launch_pass<true, false>(a, nj, grid);
-    else launch_pass<false, false>(a, nj, grid);
+    if (ddecay) launch_pass<true, false>(p, di, dj, grid);
+    else launch_pass<false, false>(p, di, dj, grid);
     int st = check_launch("linear attention");
     if (st != 0 || !ddecay) return st;
-    hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(a.heads)), dim3(kBlock), 0, ctx().stream, a.slope,
-                       ddecay, a.batch, a.heads, segs * a.tiles_j);
+    hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(a.heads)), dim3(kBlock), 0, ctx().stream,
+                       static_cast<const double*>(slope.p), ddecay, a.batch, a.heads, segs);
     return check_launch("linear attention, decay gradient");
 }
 
@@ -673,7 +1090,7 @@ int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* 
     a.kv_scale = 1.0f; a.out_scale = scale;
     if (time == 0 && !new_state) return 0;
     BSHIP_REQUIRE_PTR(decay);
-    return time <= kStepMost ? run_steps(a) : run_pass(a, nullptr);
+    return time <= kStepMost ? run_steps(a) : run_passes(Passes{{a}}, 1, nullptr);
 }
 
 int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* v, const float* decay,
@@ -699,21 +1116,29 @@ int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* 
     a.kv_scale = 1.0f; a.out_scale = scale;
     a.z = q;
     a.dfin = dnew_state;
-    if ((st = run_pass(a, ddecay)) != 0) return st;
+    if ((st = run_passes(Passes{{a}}, 1, ddecay)) != 0) return st;
     // dk: v, do, q backwards, from the transposed gradient of the new state
-    a.q = v; a.k = dout; a.v = q; a.out = dk_out;
-    a.init = dnew_state;
-    a.dfin = nullptr;
-    a.kv_scale = scale; a.out_scale = 1.0f;
-    a.reverse = 1;
-    if ((st = run_pass(a, nullptr)) != 0) return st;
-    // dv: k, q, do backwards; what is left behind the first step is the gradient of the state. This pass comes
-    // last: dstate may be dnew_state.
-    a.q = k; a.k = q; a.v = dout; a.out = dv_out;
-    a.fin = dstate;
-    a.di = static_cast<int>(dk); a.dj = static_cast<int>(dv);
-    a.si = static_cast<int>(dv); a.sj = 1;
-    return run_pass(a, nullptr);
+    Passes back = {{a, a}};
+    PassArgs& pk = back.pass[0];
+    pk.q = v; pk.k = dout; pk.v = q; pk.out = dk_out;
+    pk.init = dnew_state;
+    pk.dfin = nullptr;
+    pk.kv_scale = scale; pk.out_scale = 1.0f;
+    pk.reverse = 1;
+    // dv: k, q, do backwards; what is left behind the first step is the gradient of the state
+    PassArgs& pv = back.pass[1];
+    pv = pk;
+    pv.q = k; pv.k = q; pv.v = dout; pv.out = dv_out;
+    pv.fin = dstate;
+    pv.di = static_cast<int>(dk); pv.dj = static_cast<int>(dv);
+    pv.si = static_cast<int>(dv); pv.sj = 1;
+    // One after the other: if both passes read what the second overwrites, or only one of them has rows of fewer than
+    // four floats, which another kernel takes.
+    if ((dstate && dstate == dnew_state) || (dk < 4) != (dv < 4)) {
+        if ((st = run_passes(Passes{{pk}}, 1, nullptr)) != 0) return st;
+        return run_passes(Passes{{pv}}, 1, nullptr);
+    }
+    return run_passes(back, 2, nullptr);
 }
 
 }  // extern "C"
