@@ -30,10 +30,18 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int kPad = 128;                  // sides of the planes are multiples of this, filled with zeros
 constexpr float kScaleX = 32768.0f, kScaleP = 16384.0f;      // X and A are kept times 2^15, p times 2^14
 
-struct Planes {                            // hi at p, lo `plane` elements behind it; matrices `each` elements apart
+// A matrix (rows, 32 blocks) as two planes of blocks of 16 x 32 entries, block after block along a row of blocks. A block
+// holds its four 16 x 8 parts one after the other, each row of 8 entries (16 bytes) behind the one before: what a matrix
+// instruction takes from 64 lanes is one run of 1 KiB, in memory as in LDS, where it meets every bank once. (With plain rows,
+// whose pieces have to be turned in LDS, a product of 4096 x 4096 took 12 % more cycles.)
+struct Planes {
     _Float16* p;
-    int64_t plane, each;
-    int ld;
+    int64_t plane, each;                   // distance of the lo plane, of the matrices of a stack
+    int rows, blocks;
+    // the entry (row, k) of matrix z
+    __device__ __forceinline__ _Float16* at(unsigned z, int row, int k) const {
+        return p + z * each + (static_cast<int64_t>(row >> 4) * blocks + (k >> 5)) * 512 + (k >> 3 & 3) * 128 + (row & 15) * 8 + (k & 7);
+    }
 };
 
 __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
@@ -105,49 +113,67 @@ __global__ __launch_bounds__(kBlock) void ns_norm_kernel(UpdateArgs a) {
 // transpose. Entries outside the matrix are zeros. A matrix of zeros stays one; NaN and infinities go through.
 __global__ __launch_bounds__(kBlock) void ns_start_kernel(UpdateArgs a, Planes x, Planes xt, int tall) {
     __shared__ float tile[64][65];
-    __shared__ double s[kBlock];
+    __shared__ double s[4];
     const int64_t n = a.rows * a.cols, base = static_cast<int64_t>(blockIdx.z) * n;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
+    float u[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+        const int64_t r = r0 + x * 4 + threadIdx.x / 64, c = c0 + threadIdx.x % 64;
+        u[x] = 0.0f;
+        if (r < a.rows && c < a.cols) {
+            const int64_t at = base + r * a.cols + c;
+            u[x] = update_of(a, a.grad[at], a.velocity ? a.velocity[at] : 0.0f);
+        }
+    }
     double sum = 0.0;
     for (int i = threadIdx.x; i < a.parts; i += kBlock) sum += a.part[static_cast<int64_t>(blockIdx.z) * a.parts + i];
-    s[threadIdx.x] = sum;
-    for (int d = kBlock / 2; d > 0; d >>= 1) {
-        __syncthreads();
-        if (static_cast<int>(threadIdx.x) < d) s[threadIdx.x] += s[threadIdx.x + d];
-    }
+    for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
     __syncthreads();
-    const double inv = s[0] == 0.0 ? 0.0 : 1.0 / sqrt(s[0]);
+    sum = (s[0] + s[1]) + (s[2] + s[3]);
+    const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
     // the planes along the matrix's own rows, and those along its columns
     const Planes& along = tall ? xt : x;
     const Planes& across = tall ? x : xt;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
-    for (int e = threadIdx.x; e < 64 * 64; e += kBlock) {
-        const int64_t r = r0 + e / 64, c = c0 + e % 64;
-        float u = 0.0f;
-        if (r < a.rows && c < a.cols) {
-            const int64_t at = base + r * a.cols + c;
-            u = static_cast<float>(static_cast<double>(update_of(a, a.grad[at], a.velocity ? a.velocity[at] : 0.0f)) * inv);
-        }
-        u *= kScaleX;
-        tile[e / 64][e % 64] = u;
-        _Float16 hi, lo;
-        split(u, hi, lo);
-        _Float16* p = along.p + blockIdx.z * along.each + r * along.ld + c;
-        p[0] = hi;
-        p[along.plane] = lo;
-    }
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+        tile[x * 4 + threadIdx.x / 64][threadIdx.x % 64] = static_cast<float>(static_cast<double>(u[x]) * inv) * kScaleX;
     __syncthreads();
-    for (int e = threadIdx.x; e < 64 * 64; e += kBlock) {
-        _Float16 hi, lo;
-        split(tile[e % 64][e / 64], hi, lo);
-        _Float16* p = across.p + blockIdx.z * across.each + (c0 + e / 64) * across.ld + r0 + e % 64;
-        p[0] = hi;
-        p[across.plane] = lo;
+    // rows of 8 entries: 16 bytes of each plane
+    for (int e = threadIdx.x; e < 64 * 8; e += kBlock) {
+        const int row = e % 64, k = e / 64 * 8;
+        h8 hi, lo;
+        auto store = [&](const Planes& to, int64_t to_row, int64_t to_k) {
+            _Float16* p = to.at(blockIdx.z, static_cast<int>(to_row), static_cast<int>(to_k));
+            *reinterpret_cast<h8*>(p) = hi;
+            *reinterpret_cast<h8*>(p + to.plane) = lo;
+        };
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            _Float16 h, l;
+            split(tile[row][k + x], h, l);
+            hi[x] = h;
+            lo[x] = l;
+        }
+        store(along, r0 + row, c0 + k);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            _Float16 h, l;
+            split(tile[k + x][row], h, l);
+            hi[x] = h;
+            lo[x] = l;
+        }
+        store(across, c0 + row, r0 + k);
     }
 }
 
 struct ProductArgs {
     Planes p, q;             // C = P Q^T, both contiguous along k
     int k;                   // multiple of 32
+    int used_p, used_q;      // rows of P and Q that are not only padding
+    int tiles_p;             // tiles along the rows of P
+    unsigned tiles;          // of a matrix
     Planes c, ct;            // the result and its transpose
     UpdateArgs u;            // the last step's product goes there
     int tall;
@@ -161,154 +187,264 @@ __device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) 
 
 enum { kGram, kPoly, kNext, kLast };
 
-// C (TM x TM per workgroup of four wavefronts, each (TM / 2)^2) = P Q^T on 16 x 16 x 32 float16 matrix instructions:
-// lane l holds P[l % 16][8 (l / 16) .. + 7] and, of the result, rows 4 (l / 16) + r, column l % 16. Rows of 32 entries
-// (64 bytes) lie in LDS as four 16-byte pieces whose order is turned by the row (piece ^ (row / 4 % 4)), so that the
-// 16 lanes that read one piece of 16 rows meet all banks; loads go straight to LDS and fetch in that order.
-template <int TM, int MODE>
-__global__ __launch_bounds__(kBlock) void ns_product_kernel(ProductArgs a) {
-    constexpr int W = TM / 32;                     // tiles of 16 on a side of a wavefront's part
-    constexpr int kPlane = TM * 32;                // elements of one plane of one operand in LDS
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2][4][kPlane];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// C (T x T per workgroup) = P Q^T on 16 x 16 x 32 float16 matrix instructions: lane l holds P[l % 16][8 (l / 16) .. + 7] and, of
+// the result, rows 4 (l / 16) + r, column l % 16. WM x WN wavefronts share the tile; G such groups share the summed axis
+// (every G-th step of 32 each) and add their sums up in LDS at the end: a small tile's step is a chain of waits, which
+// other groups' steps fill. Loads go straight to LDS, a block of a plane per instruction, STAGES - 1 steps ahead.
+template <int T, int WM, int WN, int G, int STAGES, int MODE>
+__global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_product_kernel(ProductArgs a) {
+    constexpr int kWaves = WM * WN;                      // of one group
+    constexpr int X = T / WM / 16, Y = T / WN / 16;      // tiles of 16 on the sides of a wavefront's part
+    constexpr int kPlane = T * 32;                       // elements of one plane of one operand in LDS
+    constexpr int kRequests = T / 16;                    // blocks of one plane per step
+    constexpr int kLoads = 4 * kRequests / kWaves;       // of one wavefront per step
+    static_assert(4 * kRequests % kWaves == 0, "whole loads per wavefront");
+    static_assert(G == 1 || static_cast<size_t>(T) * T * 4 * G <= sizeof(_Float16) * G * STAGES * 4 * kPlane, "the sums fit");
+    __shared__ __attribute__((aligned(16))) _Float16 lds[G][STAGES][4 * kPlane];
+    const int tid = threadIdx.x, lane = tid & 63, all_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = all_wave % kWaves, group = all_wave / kWaves;
     const int l16 = lane & 15, lq = lane >> 4;
+    const int rows_p = a.p.rows, rows_q = a.q.rows;      // multiples of 128; a tile of 192 or 256 may reach behind them
+    // Consecutive workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles that lie close to each other, so
+    // that its L2 holds what they share: four rows of tiles, column by column, and four columns of the upper triangle.
+    const unsigned run = gridDim.x / 8;
+    const unsigned in_order = blockIdx.x < 8 * run ? blockIdx.x % 8 * run + blockIdx.x / 8 : blockIdx.x;
+    const unsigned z = in_order / a.tiles;
+    const int t = static_cast<int>(in_order % a.tiles);
     int bi, bj;
     if constexpr (MODE == kGram || MODE == kPoly) {
-        // tile t of the upper triangle, column by column: bj (bj + 1) / 2 <= t
-        const int t = blockIdx.x;
-        bj = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-        while ((bj + 1) * (bj + 2) / 2 <= t) ++bj;
-        while (bj * (bj + 1) / 2 > t) --bj;
-        bi = t - bj * (bj + 1) / 2;
+        // columns 4 g .. 4 g + 3 begin at tile 8 g^2 + 2 g: 4 g rows of them and a triangle
+        int g = static_cast<int>((sqrtf(32.0f * t + 4.0f) - 2.0f) * 0.0625f);
+        while (8 * (g + 1) * (g + 1) + 2 * (g + 1) <= t) ++g;
+        while (8 * g * g + 2 * g > t) --g;
+        const int width = a.tiles_p - 4 * g < 4 ? a.tiles_p - 4 * g : 4;
+        int rest = t - (8 * g * g + 2 * g);
+        if (rest < 4 * g * width) {
+            bi = rest / width;
+            bj = 4 * g + rest % width;
+        } else {
+            rest -= 4 * g * width;
+            bi = 4 * g;
+            for (int left = width; rest >= left; --left, ++bi) rest -= left;
+            bj = bi + rest;
+        }
     } else {
-        const int tiles = a.p.each / a.p.ld / TM;   // along the smaller side
-        bi = blockIdx.x % tiles;
-        bj = blockIdx.x / tiles;
+        const int tiles_q = static_cast<int>(a.tiles) / a.tiles_p, g = t / (4 * tiles_q), rest = t % (4 * tiles_q);
+        const int width = a.tiles_p - 4 * g < 4 ? a.tiles_p - 4 * g : 4;
+        bi = 4 * g + rest % width;
+        bj = rest / width;
     }
-    const _Float16* src[4] = {a.p.p + blockIdx.z * a.p.each + static_cast<int64_t>(bi) * TM * a.p.ld, nullptr,
-                              a.q.p + blockIdx.z * a.q.each + static_cast<int64_t>(bj) * TM * a.q.ld, nullptr};
-    src[1] = src[0] + a.p.plane;
-    src[3] = src[2] + a.q.plane;
 
-    auto request = [&](int buf, int k0) {
+    const _Float16* from[kLoads];                        // the same in all lanes
 #pragma unroll
-        for (int op = 0; op < 4; ++op)
+    for (int m = 0; m < kLoads; ++m) {
+        const int load = wave + m * kWaves, op = load / kRequests;
+        const Planes& side = op < 2 ? a.p : a.q;
+        const int block = (op < 2 ? bi : bj) * kRequests + load % kRequests, blocks = side.rows >> 4;
+        from[m] = side.p + z * side.each + (op & 1) * side.plane +
+                  (static_cast<int64_t>(block < blocks ? block : blocks - 1) * side.blocks + group) * 512;
+    }
+    auto request = [&](int buf, int step) {
 #pragma unroll
-            for (int m = 0; m < TM / 64; ++m) {
-                const int slot = m * kBlock + wave * kWave + lane, row = slot >> 2, piece = (slot & 3) ^ (row >> 2 & 3);
-                const int ld = op < 2 ? a.p.ld : a.q.ld;
-                load_to_lds(src[op] + static_cast<int64_t>(row) * ld + k0 + piece * 8,
-                            &lds[buf][op][(m * kBlock + wave * kWave) * 8]);
-            }
+        for (int m = 0; m < kLoads; ++m)
+            load_to_lds(from[m] + step * (512 * G) + lane * 8, &lds[group][buf][(wave + m * kWaves) * 512]);
     };
-    const int wr = (wave & 1) * (TM / 2), wc = (wave >> 1) * (TM / 2);
-    f4 acc[W][W];
+    const int wr = wave % WM * (T / WM), wc = wave / WM * (T / WN);
+    f4 acc[X][Y];
 #pragma unroll
-    for (int x = 0; x < W; ++x)
+    for (int x = 0; x < X; ++x)
 #pragma unroll
-        for (int y = 0; y < W; ++y) acc[x][y] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int y = 0; y < Y; ++y) acc[x][y] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    request(0, 0);
-    const int steps = a.k / 32;
-    for (int s = 0; s < steps; ++s) {
-        wait_until_outstanding<0>();               // this wavefront's pieces of step s are there
-        __syncthreads();                           // everybody's are, and the other buffer is free
-        if (s + 1 < steps) request((s + 1) & 1, (s + 1) * 32);
-        const _Float16* ph = lds[s & 1][0];
-        const _Float16* qh = lds[s & 1][2];
-        auto piece = [&](const _Float16* plane, int row) {
-            return *reinterpret_cast<const h8*>(plane + row * 32 + ((lq ^ (row >> 2 & 3)) * 8));
-        };
-        h8 q_hi[W], q_lo[W];
+    // steps of this group; all groups go through as many as the first, the last one perhaps without products
+    const int blocks_k = a.k / 32, steps = (blocks_k + G - 1) / G;
+    const int own = (blocks_k - group + G - 1) / G;
+    auto piece = [&](const _Float16* plane, int row) { return *reinterpret_cast<const h8*>(plane + row * 32 + lane * 8); };
+    struct Side { h8 hi[Y], lo[Y]; };
+    struct Row { h8 hi, lo; };
+    auto read_side = [&](Side& to, int buf) {
 #pragma unroll
-        for (int y = 0; y < W; ++y) {
-            q_hi[y] = piece(qh, wc + 16 * y + l16);
-            q_lo[y] = piece(qh + kPlane, wc + 16 * y + l16);
+        for (int y = 0; y < Y; ++y) {
+            to.hi[y] = piece(lds[group][buf] + 2 * kPlane, wc + 16 * y);
+            to.lo[y] = piece(lds[group][buf] + 3 * kPlane, wc + 16 * y);
         }
+    };
+    auto read_row = [&](Row& to, int buf, int x) {
+        to.hi = piece(lds[group][buf], wr + 16 * x);
+        to.lo = piece(lds[group][buf] + kPlane, wr + 16 * x);
+    };
+    // Step s with its q in `now` and its first rows of p in row[0]. Everything is read from LDS before the last X-th of the
+    // products; then the wavefronts meet, the step's buffer is given to the loads of step s + STAGES, and the first
+    // operands of step s + 1 are read while those products run.
+    Row row[2];
+    int buf = 0;                                       // s % STAGES
+    auto step = [&](int s, const Side& now, Side& next) {
+        const int after = buf + 1 == STAGES ? 0 : buf + 1;
 #pragma unroll
-        for (int x = 0; x < W; ++x) {
-            const h8 p_hi = piece(ph, wr + 16 * x + l16), p_lo = piece(ph + kPlane, wr + 16 * x + l16);
-#pragma unroll
-            for (int y = 0; y < W; ++y) {
-                acc[x][y] = mfma(p_lo, q_hi[y], acc[x][y]);
-                acc[x][y] = mfma(p_hi, q_lo[y], acc[x][y]);
-                acc[x][y] = mfma(p_hi, q_hi[y], acc[x][y]);
+        for (int x = 0; x < X; ++x) {
+            if (x + 1 < X) {
+                read_row(row[(x + 1) & 1], buf, x + 1);
+            } else if (s + 1 < steps) {
+                __builtin_amdgcn_s_waitcnt(0xc07f);    // lgkmcnt(0): this wavefront's reads have come
+                // and its pieces of step s + 1 are there: those of the steps behind it, if all of them are asked for,
+                // may be missing
+                if (s + STAGES - 1 < own) wait_until_outstanding<(STAGES - 2) * kLoads>();
+                else wait_until_outstanding<0>();
+                __builtin_amdgcn_s_barrier();          // everybody's
+                asm volatile("" ::: "memory");
+                if (s + STAGES < own) request(buf, s + STAGES);
+                read_side(next, after);
+                read_row(row[X & 1], after, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);         // the reads above are under way during the products below
+            if (G > 1 && s >= own) continue;
+            const Row& p = row[x & 1];
+#pragma unroll
+            for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.lo, now.hi[y], acc[x][y]);
+#pragma unroll
+            for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.hi, now.lo[y], acc[x][y]);
+#pragma unroll
+            for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.hi, now.hi[y], acc[x][y]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        buf = after;
+    };
+    static_assert(X % 2 == 0, "the rows of p take turns in two registers");
+    Side even, odd;
+    for (int s = 0; s < STAGES && s < own; ++s) request(s, s);
+    wait_until_outstanding<0>();
+    __syncthreads();
+    read_side(even, 0);
+    read_row(row[0], 0, 0);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, even, odd);
+        if (s + 1 < steps) step(s + 1, odd, even);
     }
 
+    // a 16 x 16 tile of the result: rows i .. i + 3, column j
+    auto finish = [&](f4 v, int i, int j) {
+        if (i >= rows_p || j >= rows_q) return;
+        if constexpr (MODE == kLast) {
+            v *= 1.0f / (kScaleP * kScaleX);
+            const int64_t base = static_cast<int64_t>(z) * a.u.rows * a.u.cols;
 #pragma unroll
-    for (int x = 0; x < W; ++x)
-#pragma unroll
-        for (int y = 0; y < W; ++y) {
-            const int64_t i = static_cast<int64_t>(bi) * TM + wr + 16 * x + 4 * lq;      // rows i .. i + 3
-            const int64_t j = static_cast<int64_t>(bj) * TM + wc + 16 * y + l16;
-            f4 v = acc[x][y];
-            if constexpr (MODE == kLast) {
-                v *= 1.0f / (kScaleP * kScaleX);
-                const int64_t base = static_cast<int64_t>(blockIdx.z) * a.u.rows * a.u.cols;
+            for (int r = 0; r < 4; ++r) {
+                const int64_t row = a.tall ? j : i + r, col = a.tall ? i + r : j;
+                if (row >= a.u.rows || col >= a.u.cols) continue;
+                float* o = a.u.out + base + row * a.u.cols + col;
+                if (a.u.add) {
+                    const float w = a.u.factor * v[r];
+                    *o = *o + w;
+                } else {
+                    *o = v[r];
+                }
+            }
+        } else {
+            if constexpr (MODE == kGram) {
+                v *= 1.0f / kScaleX;
+            } else if constexpr (MODE == kPoly) {
+                // the matrix is symmetric: rows i .. i + 3 of column j lie side by side as columns of row j
+                const _Float16* e = a.p.at(z, j, i);
+                const h4 e_hi = *reinterpret_cast<const h4*>(e), e_lo = *reinterpret_cast<const h4*>(e + a.p.plane);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int64_t row = a.tall ? j : i + r, col = a.tall ? i + r : j;
-                    if (row >= a.u.rows || col >= a.u.cols) continue;
-                    float* o = a.u.out + base + row * a.u.cols + col;
-                    if (a.u.add) {
-                        const float w = a.u.factor * v[r];
-                        *o = *o + w;
-                    } else {
-                        *o = v[r];
-                    }
+                    const float gram = static_cast<float>(e_hi[r]) + static_cast<float>(e_lo[r]);
+                    v[r] = (kB * kScaleP / kScaleX) * gram + (kC * kScaleP / (kScaleX * kScaleX)) * v[r];
+                    if (i + r == j) v[r] += kA * kScaleP;
                 }
             } else {
-                if constexpr (MODE == kGram) {
-                    v *= 1.0f / kScaleX;
-                } else if constexpr (MODE == kPoly) {
-                    const _Float16* e = a.p.p + blockIdx.z * a.p.each + i * a.p.ld + j;
+                v *= 1.0f / kScaleP;
+            }
+            h4 hi, lo;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float gram = static_cast<float>(e[r * a.p.ld]) + static_cast<float>(e[r * a.p.ld + a.p.plane]);
-                        v[r] = (kB * kScaleP / kScaleX) * gram + (kC * kScaleP / (kScaleX * kScaleX)) * v[r];
-                        if (i + r == j) v[r] += kA * kScaleP;
-                    }
-                } else {
-                    v *= 1.0f / kScaleP;
-                }
-                h4 hi, lo;
+            for (int r = 0; r < 4; ++r) {
+                _Float16 vh, vl;
+                split(v[r], vh, vl);
+                hi[r] = vh;
+                lo[r] = vl;
+            }
+            _Float16* t = a.ct.at(z, j, i);
+            *reinterpret_cast<h4*>(t) = hi;
+            *reinterpret_cast<h4*>(t + a.ct.plane) = lo;
+            // a symmetric result's diagonal tile is complete with its transpose
+            if (MODE == kNext || bi != bj) {
+                _Float16* c = a.c.at(z, i, j);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    _Float16 vh, vl;
-                    split(v[r], vh, vl);
-                    hi[r] = vh;
-                    lo[r] = vl;
-                }
-                _Float16* t = a.ct.p + blockIdx.z * a.ct.each + j * a.ct.ld + i;
-                *reinterpret_cast<h4*>(t) = hi;
-                *reinterpret_cast<h4*>(t + a.ct.plane) = lo;
-                // a symmetric result's diagonal tile is complete with its transpose
-                if (MODE == kNext || bi != bj) {
-                    _Float16* c = a.c.p + blockIdx.z * a.c.each + i * a.c.ld + j;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        c[static_cast<int64_t>(r) * a.c.ld] = hi[r];
-                        c[static_cast<int64_t>(r) * a.c.ld + a.c.plane] = lo[r];
-                    }
+                    c[8 * r] = hi[r];
+                    c[8 * r + a.c.plane] = lo[r];
                 }
             }
         }
+    };
+    if constexpr (G == 1) {
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int y = 0; y < Y; ++y) finish(acc[x][y], bi * T + wr + 16 * x + 4 * lq, bj * T + wc + 16 * y + l16);
+    } else {
+        // every group's sums, a register after the other, then each group takes every G-th tile of 16 of a wavefront's part
+        f4* sums = reinterpret_cast<f4*>(lds);
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int y = 0; y < Y; ++y) sums[((group * kWaves + wave) * X * Y + x * Y + y) * kWave + lane] = acc[x][y];
+        __syncthreads();
+        for (int n = group; n < X * Y; n += G) {
+            f4 v = sums[(wave * X * Y + n) * kWave + lane];
+#pragma unroll
+            for (int other = 1; other < G; ++other) v += sums[((other * kWaves + wave) * X * Y + n) * kWave + lane];
+            finish(v, bi * T + wr + 16 * (n / Y) + 4 * lq, bj * T + wc + 16 * (n % Y) + l16);
+        }
+    }
 }
 
+template <int T, int WM, int WN, int G, int STAGES, int MODE>
+void launch_tiles(const ProductArgs& a, unsigned count) {
+    hipLaunchKernelGGL((ns_product_kernel<T, WM, WN, G, STAGES, MODE>), dim3(a.tiles * count), dim3(WM * WN * G * kWave), 0,
+                       ctx().stream, a);
+}
+
+// The tile side: what 32 entries of the summed axis cost with one tile on every compute unit, in hundredths of a
+// microsecond, times the rounds that the tiles take. Measured (4096 x 4096: 256 against 192 and 128 for the full product
+// 336, 440 and 412 us, for the symmetric ones 280, 208 and 315; 4 x 1000 x 1000: 128 against 64 for the full product 34.5
+// and 38.7 us, for the symmetric ones 28.9 and 26.5). Tiles of 64 share a compute unit, so their rounds need not be
+// whole; where there is at most one for each, four groups share its summed axis (784 x 1200: 13 us, one group 20).
 template <int MODE>
-int launch_product(const ProductArgs& a, int tile, unsigned tiles, unsigned count) {
-    if (tile == 128)
-        hipLaunchKernelGGL((ns_product_kernel<128, MODE>), dim3(tiles, 1, count), dim3(kBlock), 0, ctx().stream, a);
-    else
-        hipLaunchKernelGGL((ns_product_kernel<64, MODE>), dim3(tiles, 1, count), dim3(kBlock), 0, ctx().stream, a);
+int launch_product(ProductArgs a, unsigned count) {
+    const int64_t cus = ctx().num_cus;
+    constexpr int kTiles[] = {256, 192, 128, 64}, kCost[] = {260, 160, 83, 30};
+    int best = 0;
+    double least = 0.0;
+    for (int n = 0; n < 4; ++n) {
+        const int64_t side = ceil_div(a.used_p, kTiles[n]), other = ceil_div(a.used_q, kTiles[n]);
+        const int64_t tiles = MODE == kGram || MODE == kPoly ? side * (side + 1) / 2 : side * other;
+        const int64_t all = tiles * count;
+        const double rounds = kTiles[n] == 64 ? static_cast<double>(all > cus ? all : cus) / cus : static_cast<double>(ceil_div(all, cus));
+        if (all > 0x7fffffff || (best && rounds * kCost[n] >= least)) continue;
+        least = rounds * kCost[n];
+        best = kTiles[n];
+        a.tiles_p = static_cast<int>(side);
+        a.tiles = static_cast<unsigned>(tiles);
+    }
+    switch (best) {
+        case 256: launch_tiles<256, 2, 4, 1, 2, MODE>(a, count); break;
+        case 192: launch_tiles<192, 2, 4, 1, 3, MODE>(a, count); break;
+        case 128: launch_tiles<128, 2, 2, 2, 2, MODE>(a, count); break;
+        case 64:
+            if (static_cast<int64_t>(a.tiles) * count > cus) launch_tiles<64, 2, 2, 1, 2, MODE>(a, count);
+            else launch_tiles<64, 2, 2, 4, 2, MODE>(a, count);
+            break;
+        default: return set_error(BSHIP_ERR_BAD_DIMENSION, "orthogonalize: the matrices exceed one launch");
+    }
     return check_launch("orthogonalize, product");
 }
 
 int orthogonal(UpdateArgs u, int64_t count, int steps) {
     const int tall = u.rows > u.cols;
     const int64_t m = ceil_div(tall ? u.cols : u.rows, kPad) * kPad, n = ceil_div(tall ? u.rows : u.cols, kPad) * kPad;
+    const int small = static_cast<int>(tall ? u.cols : u.rows), large = static_cast<int>(tall ? u.rows : u.cols);
     // planes: X, its transpose, the next X and its transpose, A, p
     const size_t x_elems = static_cast<size_t>(count) * m * n * 2, a_elems = static_cast<size_t>(count) * m * m * 2;
     int64_t parts = ceil_div(u.rows * u.cols, 16 * kBlock);
@@ -319,7 +455,7 @@ int orthogonal(UpdateArgs u, int64_t count, int steps) {
     if (st != 0) return st;
     _Float16* at = static_cast<_Float16*>(space);
     auto take = [&](int64_t rows, int64_t cols) {
-        Planes p = {at, count * rows * cols, rows * cols, static_cast<int>(cols)};
+        Planes p = {at, count * rows * cols, rows * cols, static_cast<int>(rows), static_cast<int>(cols / 32)};
         at += 2 * count * rows * cols;
         return p;
     };
@@ -334,27 +470,26 @@ int orthogonal(UpdateArgs u, int64_t count, int steps) {
                            dim3(kBlock), 0, ctx().stream, u, x, xt, tall);
         st = check_launch("orthogonalize, start");
     }
-    const int tile = count * (m / 128) * (n / 128) >= ctx().num_cus ? 128 : 64;
-    const unsigned side = static_cast<unsigned>(m / tile), triangle = side * (side + 1) / 2,
-                   all = side * static_cast<unsigned>(n / tile);
     for (int s = 0; s < steps && st == 0; ++s) {
         ProductArgs a = {};
         a.u = u;
         a.tall = tall;
         a.p = a.q = x;
-        a.k = static_cast<int>(n);
+        a.used_p = a.used_q = small;
+        a.k = (large + 31) / 32 * 32;
         a.c = a.ct = gram;
-        if ((st = launch_product<kGram>(a, tile, triangle, z)) != 0) break;
+        if ((st = launch_product<kGram>(a, z)) != 0) break;
         a.p = a.q = gram;
-        a.k = static_cast<int>(m);
+        a.k = (small + 31) / 32 * 32;
         a.c = a.ct = poly;
-        if ((st = launch_product<kPoly>(a, tile, triangle, z)) != 0) break;
+        if ((st = launch_product<kPoly>(a, z)) != 0) break;
         a.p = poly;
         a.q = xt;
+        a.used_q = large;
         a.c = y;
         a.ct = yt;
-        if (s + 1 < steps) st = launch_product<kNext>(a, tile, all, z);
-        else st = launch_product<kLast>(a, tile, all, z);
+        if (s + 1 < steps) st = launch_product<kNext>(a, z);
+        else st = launch_product<kLast>(a, z);
         Planes t = x; x = y; y = t;
         t = xt; xt = yt; yt = t;
     }
