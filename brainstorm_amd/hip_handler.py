@@ -1386,12 +1386,6 @@ class HipHandler(Handler):
     def _ptr(a):
         return a.ptr if a is not None else None
 
-    @staticmethod
-    def _overlap(a, b):
-        """Whether two dense arrays share memory."""
-        return (a is not None and b is not None and a.size > 0 and b.size > 0
-                and a.ptr < b.ptr + b.nbytes and b.ptr < a.ptr + a.nbytes)
-
     def _attention_shapes(self, op, q, k, v, decay, rows, states, lengths, others=()):
         """(time, batch, heads, dk, dv) of a linear attention call whose q, k, v lead with the axes `rows`."""
         heads = decay.size
@@ -1413,11 +1407,19 @@ class HipHandler(Handler):
             raise _mismatch(op, *[a for a, _ in others if a is not None])
         return time, batch, heads, dk, dv
 
-    def _no_overlap(self, op, outputs, inputs, allowed=()):
+    @staticmethod
+    def _no_overlap(op, outputs, inputs, allowed=()):
+        """Refuses outputs that share memory with another operand, but for the pairs (output, input) `allowed`."""
         for n, a in enumerate(outputs):
-            for b in list(inputs) + list(outputs[n + 1:]):
-                if self._overlap(a, b) and not any(a is x and b is y for x, y in allowed):
+            if a is None or not a.size:
+                continue
+            first, end = a.ptr, a.ptr + 4 * a.size
+            for b in inputs:
+                if b is not None and b.ptr < end and first < b.ptr + 4 * b.size and (a, b) not in allowed:
                     raise ValueError("%s: an output overlaps another operand" % op)
+            for b in outputs[n + 1:]:
+                if b is not None and b.ptr < end and first < b.ptr + 4 * b.size:
+                    raise ValueError("%s: two outputs overlap" % op)
 
     def linear_attention_forward(self, q, k, v, decay, out, scale=1.0, state=None, new_state=None, lengths=None):
         """Linear attention with a decay for each head over a whole sequence: S_t = decay S_(t-1) + k_t^T v_t,
