@@ -1,4 +1,4 @@
-"""The four network workloads of the benchmark configurations, on synthetic data.
+"""The four network workloads of the benchmark configurations, on synthetic data, and one more.
 
 Each builder returns ``(net, data)`` for a given handler: the network (op-trace
 drivers, see layers.py) with seeded parameters already uploaded, and the
@@ -16,13 +16,18 @@ so two handlers built with the same arguments see identical inputs and weights.
   cnn      conv5x5x32 ReLU -> maxpool 3x3/2 -> conv5x5x64 ReLU -> maxpool 3x3/2 ->
            FC1000 ReLU -> FC10 -> softmax cross entropy on 32x32x3 images
            (examples/cifar10_cnn.py:28-41); batch 100
+
+Beside them, not of the reference, one of this package's own sequence layers:
+
+  attention  FC(1000) -> N x {LinearAttention, 8 heads -> FC || gate FC -> GatedResidual} -> FC(205) -> softmax cross
+           entropy on the lstm workload's sequences
 """
 from __future__ import annotations
 
 import numpy as np
 
-from .layers import (BatchNorm, Convolution2D, Dropout, FullyConnected, Highway, Input, Loss, Lstm,
-                     Pooling2D, SoftmaxCE)
+from .layers import (BatchNorm, Convolution2D, Dropout, FullyConnected, GatedResidual, Highway, Input, LinearAttention,
+                     Loss, Lstm, Pooling2D, RmsNorm, SoftmaxCE)
 from .net import Net
 
 F32 = np.float32
@@ -101,6 +106,38 @@ def build_lstm(handler, seed=2, time_steps=100, batch=100, symbols=205, hidden=1
         ("loss", Loss(), {"default": "ce.loss"}),
     ])
     return _finish(net, data, _init_parameters(net, rng, 0.05))
+
+
+def build_attention(handler, seed=5, time_steps=100, batch=100, symbols=205, hidden=1000, heads=8, blocks=1, fused=True):
+    rng = np.random.RandomState(seed)
+    ids = rng.randint(0, symbols, (time_steps, batch, 1))
+    onehot = np.zeros((time_steps, batch, symbols), dtype=F32)     # like data_iterators.OneHot
+    np.put_along_axis(onehot, ids, 1.0, axis=2)
+    data = {"default": onehot, "targets": ids.astype(F32)}
+    layers = [("Input", Input({"default": (symbols,), "targets": (1,)}), {}),
+              ("embed", FullyConnected(hidden, "linear", fused=fused), {"default": "Input.default"}),
+              ("norm", RmsNorm(), {"default": "embed.default"})]
+    normed, residual = "norm.default", "embed.default"
+    for k in range(blocks):
+        layers += [
+            ("attend%d" % k, LinearAttention(hidden, heads), {"default": normed}),
+            ("mix%d" % k, FullyConnected(hidden, "linear", fused=fused), {"default": "attend%d.default" % k}),
+            ("gate%d" % k, FullyConnected(hidden, "linear", fused=fused), {"default": normed}),
+            ("end%d" % k, GatedResidual("swish"), {"block": "mix%d.default" % k, "gate": "gate%d.default" % k,
+                                                   "x": residual}),
+        ]
+        normed, residual = "end%d.default" % k, "end%d.residual" % k
+    layers += [
+        ("out", FullyConnected(symbols, "linear", fused=fused), {"default": normed}),
+        ("ce", SoftmaxCE(fused=fused), {"default": "out.default", "targets": "Input.targets"}),
+        ("loss", Loss(), {"default": "ce.loss"}),
+    ]
+    net = Net(handler, layers)
+    flat = _init_parameters(net, rng, 0.05, special={"weight": 1.0, "post": 1.0, "pre": 1.0})
+    for name, (a, b, _) in net.parameter_slices().items():
+        if name.endswith(".decay"):                # memories of 8 to 128 steps: g = 1 - 1 / memory
+            flat[a:b] = np.log(2.0 ** np.linspace(3, 7, b - a) - 1)
+    return _finish(net, data, flat)
 
 
 def build_highway(handler, seed=3, blocks=50, batch=2048, width=4096, classes=10, fused=False,

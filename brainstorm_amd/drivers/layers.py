@@ -679,6 +679,104 @@ class Highway(Layer):
         _h.mult_add_tt(tmp, dy, out=dT)
 
 
+class RmsNorm(Layer):
+    """out = weight * x / rms(x) over the features: the norm before the first block of GatedResidual blocks. No
+    counterpart in the reference; needs a handler with rms_norm_forward."""
+
+    def __init__(self, epsilon=1.0e-6):
+        self.epsilon = epsilon
+
+    def setup(self, in_shapes):
+        shape = in_shapes["default"].feature_shape
+        return OrderedDict(default=Buf(shape)), OrderedDict(weight=(_prod(shape),)), OrderedDict()
+
+    def forward_pass(self, buffers, training_pass=True):
+        self.handler.rms_norm_forward(flatten_time_and_features(buffers.inputs["default"]), buffers.parameters["weight"],
+                                      flatten_time_and_features(buffers.outputs["default"]), epsilon=self.epsilon)
+
+    def backward_pass(self, buffers):
+        self.handler.rms_norm_backward(
+            flatten_time_and_features(buffers.inputs["default"]), buffers.parameters["weight"],
+            flatten_time_and_features(buffers.output_deltas["default"]),
+            flatten_time_and_features(buffers.input_deltas["default"]), buffers.gradients["weight"], epsilon=self.epsilon)
+
+
+class GatedResidual(Layer):
+    """The end of a block: y = residual_scale * x + act(gate) * post * block / rms(block), and the norm before the next
+    block, pre * y / rms(y), with inputs 'block', 'gate' (before its activation) and 'x'. Outputs: 'default', the
+    normed one, and 'residual', y. No counterpart in the reference (the Highway layer's relative); needs a handler
+    with gated_residual_forward."""
+
+    def __init__(self, activation="swish", residual_scale=1.0, epsilon=1.0e-6):
+        self.activation = activation
+        self.residual_scale = residual_scale
+        self.epsilon = epsilon
+
+    def setup(self, in_shapes):
+        shape = in_shapes["x"].feature_shape
+        parameters = OrderedDict([("post", (_prod(shape),)), ("pre", (_prod(shape),))])
+        return OrderedDict([("default", Buf(shape)), ("residual", Buf(shape))]), parameters, OrderedDict()
+
+    def forward_pass(self, buffers, training_pass=True):
+        block, gate, x = (flatten_time_and_features(buffers.inputs[n]) for n in ("block", "gate", "x"))
+        h, y = (flatten_time_and_features(buffers.outputs[n]) for n in ("default", "residual"))
+        self.handler.gated_residual_forward(self.activation, block, gate, x, buffers.parameters["post"],
+                                            buffers.parameters["pre"], y, h, residual_scale=self.residual_scale,
+                                            epsilon=self.epsilon)
+
+    def backward_pass(self, buffers):
+        block, gate = (flatten_time_and_features(buffers.inputs[n]) for n in ("block", "gate"))
+        dblock, dgate, dx = (flatten_time_and_features(buffers.input_deltas[n]) for n in ("block", "gate", "x"))
+        dh, dy = (flatten_time_and_features(buffers.output_deltas[n]) for n in ("default", "residual"))
+        self.handler.gated_residual_backward(
+            self.activation, block, gate, buffers.parameters["post"], buffers.parameters["pre"],
+            flatten_time_and_features(buffers.outputs["residual"]), dy, dh, dblock, dgate, dx,
+            buffers.gradients["post"], buffers.gradients["pre"], residual_scale=self.residual_scale, epsilon=self.epsilon)
+
+
+class LinearAttention(Layer):
+    """A recurrent layer of heads with a matrix each as their state: S_t = g S_(t-1) + k_t^T v_t, out_t = q_t S_t / sqrt(d),
+    with q, k, v = x Wq^T, x Wk^T, x Wv^T and the heads' decays g = sigmoid(decay). No counterpart in the reference
+    (the Lstm layer's relative); needs a handler with linear_attention_forward."""
+
+    def __init__(self, size, heads):
+        self.size = int(size)
+        self.heads = int(heads)
+        if self.size % self.heads:
+            raise ValueError("%d features are not those of %d heads" % (self.size, self.heads))
+        self.scale = (self.size // self.heads) ** -0.5
+
+    def setup(self, in_shapes):
+        in_size = _prod(in_shapes["default"].feature_shape)
+        parameters = OrderedDict([(w, (self.size, in_size)) for w in ("Wq", "Wk", "Wv")] + [("decay", (self.heads,))])
+        internals = OrderedDict([(n, Buf((self.size,))) for n in ("q", "k", "v")]
+                                + [(n, Buf((self.size,), backward_only=True)) for n in ("dq", "dk", "dv")]
+                                + [("g", Buf((self.heads,), scales=""))])
+        return OrderedDict(default=Buf((self.size,))), parameters, internals
+
+    def forward_pass(self, buffers, training_pass=True):
+        _h = self.handler
+        x = flatten_time_and_features(buffers.inputs["default"])
+        q, k, v, g = (buffers.internals[n] for n in ("q", "k", "v", "g"))
+        for w, a in (("Wq", q), ("Wk", k), ("Wv", v)):
+            _h.dot_mm(x, buffers.parameters[w], flatten_time(a), transb=True)
+        _h.sigmoid(buffers.parameters["decay"], g)
+        _h.linear_attention_forward(q, k, v, g, buffers.outputs["default"], scale=self.scale)
+
+    def backward_pass(self, buffers):
+        _h = self.handler
+        x = flatten_time_and_features(buffers.inputs["default"])
+        dx = flatten_time_and_features(buffers.input_deltas["default"])
+        q, k, v, dq, dk, dv, g = (buffers.internals[n] for n in ("q", "k", "v", "dq", "dk", "dv", "g"))
+        ddecay = buffers.gradients["decay"]
+        _h.linear_attention_backward(q, k, v, g, buffers.output_deltas["default"], dq, dk, dv, ddecay, scale=self.scale)
+        _h.sigmoid_deriv(None, g, ddecay, ddecay)
+        for w, d in (("Wq", dq), ("Wk", dk), ("Wv", dv)):
+            d = flatten_time(d)
+            _h.dot_mm(d, x, buffers.gradients[w], transa=True)
+            _h.dot_add_mm(d, buffers.parameters[w], dx)
+
+
 def _conv_out(size, kernel, padding, stride):
     return (size + 2 * padding - kernel) // stride + 1
 

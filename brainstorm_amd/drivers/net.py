@@ -244,3 +244,44 @@ class MomentumStepper:
         if getattr(self, "_recorded", None) is not None:
             self._recorded.release()
             self._recorded = None
+
+
+class OrthogonalStepper(MomentumStepper):
+    """A MomentumStepper whose weight matrices take orthogonalised steps (handler.orthogonal_update): every parameter
+    with two or more axes as the matrix (first axis, all others), equal matrices that lie behind each other in the
+    parameter vector in one call. Parameters with one axis, biases and the like, take momentum steps with
+    ``vector_learning_rate``. No counterpart in the reference."""
+
+    def __init__(self, learning_rate=0.02, momentum=0.95, vector_learning_rate=0.01, nesterov=True, iterations=5):
+        super().__init__(learning_rate, momentum, scale_learning_rate=False, fused=True)
+        self.vector_learning_rate = vector_learning_rate
+        self.nesterov = nesterov
+        self.iterations = iterations
+        self.groups = None
+
+    def start(self, net):
+        super().start(net)
+        # runs of the parameter vector: [first, end, shape of the matrices or None]
+        runs = []
+        for first, end, shape in net.parameter_slices().values():
+            matrix = (int(shape[0]), _prod(shape[1:])) if len(shape) >= 2 and first < end else None
+            if runs and runs[-1][1] == first and runs[-1][2] == matrix:
+                runs[-1][1] = end
+            elif first < end:
+                runs.append([first, end, matrix])
+        self.groups = runs
+
+    def run(self):
+        net = self.net
+        net.forward_pass(training_pass=True)
+        net.backward_pass()
+        h = net.handler
+        for first, end, matrix in self.groups:
+            g, v, p = (a[first:end] for a in (net.gradients, self.velocity, net.parameters))
+            if matrix is None:
+                h.momentum_update(self.momentum, -self.vector_learning_rate, g, v, p)
+            else:
+                shape = ((end - first) // _prod(matrix),) + matrix
+                h.orthogonal_update(self.momentum, -self.learning_rate, g.reshape(shape), v.reshape(shape),
+                                    p.reshape(shape), steps=self.iterations, nesterov=self.nesterov)
+        net.apply_weight_modifiers()

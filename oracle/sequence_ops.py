@@ -1,6 +1,10 @@
 """Linear attention with a decay, the gated residual with its norms, and Newton-Schulz orthogonalisation in
-plain NumPy, float64 throughout, written from the definitions: what the tests of the kernels compare with."""
+plain NumPy, float64 throughout, written from the definitions: what the tests of the kernels compare with. TEST
+INFRASTRUCTURE, like the rest of this package; ``SequenceRefHandler`` gives the oracle handler these operators, so
+that networks with them run on it."""
 import numpy as np
+
+from .numpy_ref_handler import NumpyRefHandler
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -154,3 +158,64 @@ def orthogonal_update(momentum, neg_learning_rate, gradients, velocity, paramete
     u = g + momentum * v if nesterov else v
     rows, cols = p.shape[-2:]
     return v, p + neg_learning_rate * np.sqrt(max(1.0, rows / cols)) * orthogonalize(u, steps)
+
+
+class SequenceRefHandler(NumpyRefHandler):
+    """The oracle handler with HipHandler's sequence, norm and update operators (same signatures), in 64 bits and
+    rounded once."""
+
+    def linear_attention_forward(self, q, k, v, decay, out, scale=1.0, state=None, new_state=None, lengths=None):
+        o, s = linear_attention(q, k, v, decay, scale, state, lengths)
+        out[:] = o.reshape(out.shape)
+        if new_state is not None:
+            new_state[:] = s.reshape(new_state.shape)
+
+    def linear_attention_step(self, q, k, v, decay, state, out, scale=1.0):
+        o, s = linear_attention(q[None], k[None], v[None], decay, scale, state)
+        out[:] = o.reshape(out.shape)
+        state[:] = s.reshape(state.shape)
+
+    def linear_attention_backward(self, q, k, v, decay, dout, dq, dk, dv, ddecay=None, scale=1.0, state=None,
+                                  dnew_state=None, dstate=None, lengths=None):
+        results = linear_attention_gradients(q, k, v, decay, dout, scale, state, dnew_state, lengths)
+        for to, x in zip((dq, dk, dv, ddecay, dstate), results):
+            if to is not None:
+                to[:] = x.reshape(to.shape)
+
+    def gated_residual_forward(self, activation, block, gate, x, post_weight, pre_weight, y, h, residual_scale=1.0,
+                               epsilon=1e-6):
+        y64, h64 = gated_residual(activation, block, gate, x, post_weight, pre_weight, residual_scale, epsilon)
+        y[:] = y64
+        if pre_weight is not None:
+            h[:] = h64
+
+    def gated_residual_backward(self, activation, block, gate, post_weight, pre_weight, y, dy, dh, dblock, dgate, dx,
+                                dpost_weight, dpre_weight, residual_scale=1.0, epsilon=1e-6, accumulate=True):
+        results = gated_residual_gradients(activation, block, gate, post_weight, pre_weight, y, dy,
+                                           dh if pre_weight is not None else None, residual_scale, epsilon)
+        for to, name in ((dblock, "dblock"), (dgate, "dgate"), (dx, "dx")):
+            if to is not None:
+                to[:] = results[name] + (to if accumulate else 0)
+        for to, name in ((dpost_weight, "dpost"), (dpre_weight, "dpre")):
+            if to is not None:
+                to[:] = results[name].reshape(to.shape)
+
+    def rms_norm_forward(self, x, weight, out, epsilon=1e-6):
+        out[:] = gated_residual("linear", None, None, x, None, weight, epsilon=epsilon)[1]
+
+    def rms_norm_backward(self, x, weight, dout, dx, dweight, epsilon=1e-6, accumulate=True):
+        results = gated_residual_gradients("linear", None, None, None, weight, x, None, dout, epsilon=epsilon)
+        dx[:] = results["dx"] + (dx if accumulate else 0)
+        dweight[:] = results["dpre"].reshape(dweight.shape)
+
+    def orthogonalize(self, m, out, steps=5):
+        out[:] = orthogonalize(m, steps)
+
+    def orthogonal_update(self, momentum, neg_learning_rate, gradients, velocity, parameters, steps=5, nesterov=True):
+        velocity[:], parameters[:] = orthogonal_update(momentum, neg_learning_rate, gradients, velocity, parameters,
+                                                       steps, nesterov)
+
+    def momentum_update(self, momentum, neg_learning_rate, gradients, velocity, parameters):
+        self.mult_st(momentum, velocity, out=velocity)
+        self.mult_add_st(neg_learning_rate, gradients, out=velocity)
+        self.add_tt(velocity, parameters, out=parameters)
