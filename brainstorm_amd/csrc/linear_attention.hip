@@ -584,21 +584,146 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
 
 // Short sequences without a state before or behind them: all scores are formed, none goes through a state. With d
 // features a position costs 4 d (T / 2) operations instead of the 4 d^2 + 128 d of a pass in chunks.
-//
-// A wavefront has the 16 positions of one tile: q as operands in registers, the sums over v as accumulators. The
+constexpr int kAllScores = 128;        // positions that the kernels below cover
+
+// 32 rows of d floats on their way from memory into LDS, a thread's pieces of 16 bytes. Loads are made without conditions:
+// rows behind the last are taken from it, and become zeros in LDS.
+template <int N, int THREADS>
+struct Rows {
+    static constexpr int kRow = 4 * N, kPieces = kChunk * kRow, kLoads = (kPieces + THREADS - 1) / THREADS, LD = 16 * N + 4;
+    f4 x[kLoads];
+
+    // column of piece e: the last one of a row whose length is no multiple of 4 ends with the row
+    static __device__ __forceinline__ int column(int e, int d) {
+        const int col = e % kRow * 4;
+        return col >= d ? 0 : col + 4 > d ? d - 4 : col;
+    }
+    __device__ __forceinline__ void fetch(const float* p, int64_t step, int d, int first, int len) {
+        const int tid = form_again(threadIdx.x);
+#pragma unroll
+        for (int m = 0; m < kLoads; ++m) {
+            const int e = tid + m * THREADS, row = first + e / kRow % kChunk;
+            x[m] = *reinterpret_cast<const f4u*>(p + (row < len ? row : len - 1) * step + column(e, d));
+        }
+    }
+    __device__ __forceinline__ void put(float* to, int d, int first, int len) const {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int m = 0; m < kLoads; ++m) {
+            const int e = tid + m * THREADS;
+            if ((kPieces % THREADS && e >= kPieces) || e % kRow * 4 >= d) continue;
+            const f4 y = first + e / kRow < len ? x[m] : f4{0.0f, 0.0f, 0.0f, 0.0f};
+            float* at = to + e / kRow * LD + column(e, d);
+            if (d & 3) {                           // pieces that do not begin at multiples of 16 bytes
+#pragma unroll
+                for (int r = 0; r < 4; ++r) at[r] = y[r];
+            } else {
+                *reinterpret_cast<f4*>(at) = y;
+            }
+        }
+    }
+};
+
+// A row's pieces 16 it + 4 lq as operands; 0 behind its d floats.
+template <int N>
+__device__ __forceinline__ void read_operand(f4 (&to)[N], const float* row, int d, int lq) {
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+        const int col = 16 * it + 4 * lq;
+        to[it] = *reinterpret_cast<const f4u*>(row + (col + 4 <= d ? col : d - 4));
+    }
+    // the piece with the row's end was read up to it
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+        const int over = 16 * it + 4 * lq + 4 - d;
+        f4 x = to[it];
+        if (over == 1) x = f4{x[1], x[2], x[3], 0.0f};
+        if (over == 2) x = f4{x[2], x[3], 0.0f, 0.0f};
+        if (over == 3) x = f4{x[3], 0.0f, 0.0f, 0.0f};
+        if (over > 3) x = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        to[it] = x;
+    }
+}
+
+// 16 rows in LDS times one column: D[16 rows][column] of lane (lq, l16): rows 4 lq + r, the own position as column l16.
+template <int N>
+__device__ __forceinline__ f4 scores(const float* rows, const f4 (&own)[N], int l16, int lq) {
+    const float* p = rows + l16 * (16 * N + 4) + 4 * lq;
+    f4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s, x[2];
+    x[0] = *reinterpret_cast<const f4*>(p);
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+        if (it + 1 < N) x[(it + 1) & 1] = *reinterpret_cast<const f4*>(p + 16 * (it + 1));
+        one_step_ahead();
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            s = mfma(x[it & 1][r], own[it][r], s);
+            s2 = mfma(x[it & 1][r + 1], own[it][r + 1], s2);
+        }
+    }
+    return s + s2;
+}
+
+// acc[j] += sum over 16 rows y in LDS of rows[y][j] w[y], w as `scores` leaves it. On the diagonal a weight of 0 would carry a
+// NaN or an infinity to positions that do not see it: such values are left out of the products and added one by one to the
+// positions that do, which are those from y on (EARLIER = false), or up to y.
+template <int N, int LD, bool EARLIER>
+__device__ __forceinline__ void add_rows(f4 (&acc)[N], const float (&w)[4], const float* rows, bool diagonal, int l16, int lq) {
+    const float* p = rows + 4 * lq * LD + l16;
+    float x[2][4];
+    auto read = [&](int jt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[jt & 1][r] = p[r * LD + 16 * jt];
+    };
+    read(0);
+    float nothing = 0.0f;                          // a NaN if a value is not finite
+#pragma unroll
+    for (int jt = 0; jt < N; ++jt) {
+        if (jt + 1 < N) read(jt + 1);
+        one_step_ahead();
+        if (diagonal)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                nothing += 0.0f * x[jt & 1][r];
+                x[jt & 1][r] = __builtin_isfinite(x[jt & 1][r]) ? x[jt & 1][r] : 0.0f;
+            }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[jt] = mfma(x[jt & 1][r], w[r], acc[jt]);
+    }
+    if (__all(nothing == 0.0f)) return;
+    for (int y = 0; y < 16; ++y) {
+        // the weight of row y and this lane's column: lane 16 (y / 4) + l16, element y % 4
+        const int from = 16 * (y >> 2) + l16;
+        float wy = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float w0 = __shfl(w[r], from);
+            if ((y & 3) == r) wy = w0;
+        }
+        if (EARLIER ? l16 > y : l16 < y) continue;
+#pragma unroll
+        for (int jt = 0; jt < N; ++jt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float xy = rows[y * LD + 16 * jt + 4 * lq + r];
+                if (!__builtin_isfinite(xy)) acc[jt][r] += wy * xy;
+            }
+    }
+}
+
+// Forwards. A wavefront has the 16 positions of one tile: q as operands in registers, the sums over v as accumulators. The
 // rows of k and v come through LDS in steps of 32 positions; a tile of scores (b, a) is at once the operand of its
 // product with v. Tile n has n + 1 tiles of scores: wavefronts s and s + 4, which share a SIMD, take tiles whose work adds
 // up to the same.
-constexpr int kAllScores = 128;        // positions that eight wavefronts cover
-template <int NI, int NJ, bool TAN>
-__global__ __launch_bounds__(8 * kWave, TAN ? 2 : 4) void la_scores_kernel(Passes passes) {
-    constexpr int LD = 16 * NI + 4, LDV = 16 * NJ + 4, kThreads = 8 * kWave;
-    constexpr int kRowsK = kChunk * LD, kRowsV = kChunk * LDV;
+template <int NI, int NJ>
+__global__ __launch_bounds__(8 * kWave, 4) void la_scores_kernel(PassArgs a) {
+    constexpr int kThreads = 8 * kWave;
+    using RowsK = Rows<NI, kThreads>;
+    using RowsV = Rows<NJ, kThreads>;
+    constexpr int kRowsK = kChunk * RowsK::LD, kRowsV = kChunk * RowsV::LD;
     __shared__ __attribute__((aligned(16))) float k_all[2 * kRowsK], v_all[2 * kRowsV];
-    __shared__ float pk[kAllScores], sk[TAN ? kAllScores : 1];       // kv_scale times g^n and n g^(n-1)
-    __shared__ double part_s[8];
+    __shared__ float pk[kAllScores];                                 // kv_scale times g^n
 
-    const PassArgs& a = passes.pass[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lq = lane >> 4;
     const int64_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
@@ -606,193 +731,197 @@ __global__ __launch_bounds__(8 * kWave, TAN ? 2 : 4) void la_scores_kernel(Passe
     const int tiles = (len + 15) >> 4;
     const int mine = wave < 4 ? tiles - 1 - wave : wave - 4 - (8 - tiles);       // the tile of this wavefront, or < 0
     const int p = mine >= 0 ? 16 * mine + l16 : 0;                               // this lane's position as a column
-    // position p is time p forwards, len - 1 - p backwards
     const int64_t step_i = a.batch * a.heads * a.di, step_j = a.batch * a.heads * a.dj;
-    auto time_of = [&](int x) { return a.reverse ? len - 1 - x : x; };
-
-    // ---- rows of the next 32 positions, on their way from memory; rows behind the last are taken from the last
-    constexpr int kPiecesK = kChunk * 4 * NI, kPiecesV = kChunk * 4 * NJ;
-    constexpr int kLoadsK = (kPiecesK + kThreads - 1) / kThreads, kLoadsV = (kPiecesV + kThreads - 1) / kThreads;
-    auto piece_col = [](int e, int per_row, int d) {
-        const int col = e % per_row * 4;
-        return col >= d ? 0 : col + 4 > d ? d - 4 : col;
-    };
-    f4 k_n[kLoadsK], v_n[kLoadsV];
-    auto fetch = [&](int first) {
-        const int tid = form_again(threadIdx.x);
-#pragma unroll
-        for (int m = 0; m < kLoadsK; ++m) {
-            const int e = tid + m * kThreads, x = first + e / (4 * NI) % kChunk;
-            k_n[m] = *reinterpret_cast<const f4u*>(a.k + time_of(x < len ? x : len - 1) * step_i + bh * a.di + piece_col(e, 4 * NI, a.di));
-        }
-#pragma unroll
-        for (int m = 0; m < kLoadsV; ++m) {
-            const int e = tid + m * kThreads, x = first + e / (4 * NJ) % kChunk;
-            v_n[m] = *reinterpret_cast<const f4u*>(a.v + time_of(x < len ? x : len - 1) * step_j + bh * a.dj + piece_col(e, 4 * NJ, a.dj));
-        }
-    };
-    auto put = [&](float* to, const f4& x, int e, int pieces, int per_row, int d, int ld) {
-        if (e >= pieces || e % per_row * 4 >= d) return;
-        float* at = to + e / per_row * ld + piece_col(e, per_row, d);
-        if (d & 3) {                           // pieces that do not begin at multiples of 16 bytes
-#pragma unroll
-            for (int r = 0; r < 4; ++r) at[r] = x[r];
-        } else {
-            *reinterpret_cast<f4*>(at) = x;
-        }
-    };
+    const float *k = a.k + bh * a.di, *v = a.v + bh * a.dj;
+    RowsK k_n;
+    RowsV v_n;
     f4 qf[NI];
     if (len > 0) {
-        fetch(0);
-        const float* q = a.q + time_of(p < len ? p : len - 1) * step_i + bh * a.di;
-#pragma unroll
-        for (int it = 0; it < NI; ++it) {
-            const int col = 16 * it + 4 * lq;
-            qf[it] = *reinterpret_cast<const f4u*>(q + (col + 4 <= a.di ? col : a.di - 4));
-        }
-        // the piece with the row's end was read up to it; what is behind the end is 0
-#pragma unroll
-        for (int it = 0; it < NI; ++it) {
-            const int over = 16 * it + 4 * lq + 4 - a.di;
-            f4 x = qf[it];
-            if (over == 1) x = f4{x[1], x[2], x[3], 0.0f};
-            if (over == 2) x = f4{x[2], x[3], 0.0f, 0.0f};
-            if (over == 3) x = f4{x[3], 0.0f, 0.0f, 0.0f};
-            if (over > 3) x = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            qf[it] = x;
-        }
+        k_n.fetch(k, step_i, a.di, 0, len);
+        v_n.fetch(v, step_j, a.dj, 0, len);
+        read_operand(qf, a.q + (p < len ? p : len - 1) * step_i + bh * a.di, a.di, lq);
     }
-    if (tid < kAllScores) {
-        const double g = a.decay[h];
-        pk[tid] = a.kv_scale * static_cast<float>(power(g, tid));
-        if (TAN) sk[tid] = tid ? a.kv_scale * static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
-    }
+    if (tid < kAllScores) pk[tid] = a.kv_scale * static_cast<float>(power(static_cast<double>(a.decay[h]), tid));
     // columns that a row does not have: zeros, which nothing overwrites
     for (int e = tid * 4; e < 2 * kRowsK; e += kThreads * 4) *reinterpret_cast<f4*>(k_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int e = tid * 4; e < 2 * kRowsV; e += kThreads * 4) *reinterpret_cast<f4*>(v_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    f4 o[NJ], dz[TAN ? NJ : 1];
+    f4 o[NJ];
 #pragma unroll
-    for (int jt = 0; jt < NJ; ++jt) {
-        o[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (TAN) dz[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int jt = 0; jt < NJ; ++jt) o[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
 
     for (int first = 0; first < len; first += kChunk) {
         float* const k_s = k_all + (first / kChunk & 1) * kRowsK;
         float* const v_s = v_all + (first / kChunk & 1) * kRowsV;
-#pragma unroll
-        for (int m = 0; m < kLoadsK; ++m) put(k_s, k_n[m], tid + m * kThreads, kPiecesK, 4 * NI, a.di, LD);
-#pragma unroll
-        for (int m = 0; m < kLoadsV; ++m) put(v_s, v_n[m], tid + m * kThreads, kPiecesV, 4 * NJ, a.dj, LDV);
+        k_n.put(k_s, a.di, first, len);
+        v_n.put(v_s, a.dj, first, len);
         __syncthreads();                       // two buffers: nobody reads the ones before the last any more
-        if (first + kChunk < len) fetch(first + kChunk);
+        if (first + kChunk < len) {
+            k_n.fetch(k, step_i, a.di, first + kChunk, len);
+            v_n.fetch(v, step_j, a.dj, first + kChunk, len);
+        }
         for (int x = first; x < first + kChunk && x <= 16 * mine; x += 16) {
-            const float* kp = k_s + (x - first + l16) * LD + 4 * lq;
-            const float* vp = v_s + (x - first + 4 * lq) * LDV + l16;
-            f4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s, kf[2];
-            kf[0] = *reinterpret_cast<const f4*>(kp);
-#pragma unroll
-            for (int it = 0; it < NI; ++it) {
-                if (it + 1 < NI) kf[(it + 1) & 1] = *reinterpret_cast<const f4*>(kp + 16 * (it + 1));
-                one_step_ahead();
-#pragma unroll
-                for (int r = 0; r < 4; r += 2) {
-                    s = mfma(kf[it & 1][r], qf[it][r], s);
-                    s2 = mfma(kf[it & 1][r + 1], qf[it][r + 1], s2);
-                }
-            }
-            const int distance = 16 * mine + l16 - x - 4 * lq;           // a - b of r = 0
-            float w[4], dw[4];
+            const f4 s = scores<NI>(k_s + (x - first) * RowsK::LD, qf, l16, lq);
+            float w[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int e = distance - r;                              // below 0: 0 whatever the score
-                const float y = s[r] + s2[r];
-                w[r] = e >= 0 ? y * pk[e] : 0.0f;
-                dw[r] = TAN && e >= 0 ? y * sk[e] : 0.0f;
+                const int e = p - x - 4 * lq - r;                        // a - b; below 0: 0 whatever the score
+                w[r] = e >= 0 ? s[r] * pk[e] : 0.0f;
             }
-            float vf[2][4];
-            auto read = [&](int jt) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) vf[jt & 1][r] = vp[r * LDV + 16 * jt];
-            };
-            read(0);
-            float nothing = 0.0f;                                        // a NaN if a value of v is not finite
-#pragma unroll
-            for (int jt = 0; jt < NJ; ++jt) {
-                if (jt + 1 < NJ) read(jt + 1);
-                one_step_ahead();
-                // on the diagonal a score of 0 would carry a NaN or an infinity to positions before it
-                if (x == 16 * mine)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        nothing += 0.0f * vf[jt & 1][r];
-                        vf[jt & 1][r] = __builtin_isfinite(vf[jt & 1][r]) ? vf[jt & 1][r] : 0.0f;
-                    }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    o[jt] = mfma(vf[jt & 1][r], w[r], o[jt]);
-                    if (TAN) dz[jt] = mfma(vf[jt & 1][r], dw[r], dz[jt]);
-                }
-            }
-            if (!__all(nothing == 0.0f)) {                               // such values reach their own and later positions
-                for (int y = 0; y < 16; ++y) {
-                    // the score of b = y, a = this lane's: lane 16 (y / 4) + l16, element y % 4
-                    const int from = 16 * (y >> 2) + l16;
-                    float wy = 0.0f, dwy = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float w0 = __shfl(w[r], from), w1 = __shfl(dw[r], from);
-                        if ((y & 3) == r) {
-                            wy = w0;
-                            dwy = w1;
-                        }
-                    }
-                    if (l16 < y) continue;
-#pragma unroll
-                    for (int jt = 0; jt < NJ; ++jt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float vy = v_s[(x - first + y) * LDV + 16 * jt + 4 * lq + r];
-                            if (__builtin_isfinite(vy)) continue;
-                            o[jt][r] += wy * vy;
-                            if (TAN) dz[jt][r] += dwy * vy;
-                        }
-                }
-            }
+            add_rows<NJ, RowsV::LD, false>(o, w, v_s + (x - first) * RowsV::LD, x == 16 * mine, l16, lq);
         }
     }
 
     // lane: position p, columns 16 jt + 4 lq .. + 3
-    double slope = 0.0;
-    if (mine >= 0 && p < len) {
-        const int64_t row = time_of(p) * step_j + bh * a.dj;
+    if (mine >= 0 && p < len)
 #pragma unroll
         for (int jt = 0; jt < NJ; ++jt) {
-            const int col = 16 * jt + 4 * lq, left = a.dj - col;
-            if (left <= 0) continue;
-            store4(a.out + row + col, a.out_scale * o[jt], left);
-            if (TAN) {
-                const f4 z = load4(a.z + row + col, left);
-                float s = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r < left) s += z[r] * dz[jt][r];
-                slope += static_cast<double>(a.out_scale * s);
-            }
+            const int col = 16 * jt + 4 * lq;
+            store4(a.out + p * step_j + bh * a.dj + col, a.out_scale * o[jt], a.dj - col);
         }
-    }
     // rows behind the sequence's end
     for (int64_t x = len + wave; x < a.time; x += 8)
         for (int j = lane; j < a.dj; j += kWave) a.out[x * step_j + bh * a.dj + j] = 0.0f;
-    if constexpr (TAN) {
+}
+
+// Backwards: all gradients from each score formed once. s_ab = q_a . k_b and p_ab = do_a . v_b (b <= a, W_ab = g^(a-b)) give
+//   dv_b = scale sum_a W s do_a,   dk_b = scale sum_a W p q_a,   dq_a = scale sum_b W p k_b,
+//   ddecay = scale sum (a-b) g^(a-b-1) s p,
+// five products of tiles where the passes one by one take seven and read ten arrays instead of five.
+//
+// First the keys' gradients: wavefronts 2 n and 2 n + 1 have the positions of tile n as columns, one with k and the sums of dv,
+// one with v and the sums of dk, while the rows of q and do come through LDS; both leave their scores there. Then the
+// queries': wavefronts 2 n and 2 n + 1 have half of the features of dq each, k comes through LDS, and the scores are
+// read back with rows and columns exchanged. Consecutive tiles lie on different SIMDs, so that the tiles that a step of 32
+// positions reaches are spread evenly over them, but for the last ones.
+struct BackArgs {
+    const float *q, *k, *v, *dout, *decay, *lengths;
+    float *dq, *dk, *dv;
+    double* slope;                     // one partial sum per sequence, or NULL
+    int64_t time, batch, heads;
+    int di, dj;
+    float scale;
+};
+
+template <int N, int TILES>
+__global__ __launch_bounds__(2 * TILES * kWave, TILES == 4 && N == 8 ? 2 : 4) void la_scores_bwd_kernel(BackArgs a) {
+    constexpr int kThreads = 2 * TILES * kWave, kHalf = N / 2;
+    using R = Rows<N, kThreads>;
+    constexpr int LD = R::LD, kRows = kChunk * LD;
+    constexpr int kLD = 20, kTile = 16 * kLD, kPairs = TILES * (TILES + 1) / 2;      // tiles of scores: rows a, columns b
+    __shared__ __attribute__((aligned(16))) float q_all[2 * kRows], do_all[2 * kRows];
+    __shared__ __attribute__((aligned(16))) float s_all[kPairs * kTile], p_all[kPairs * kTile];
+    __shared__ float pk[16 * TILES], sk[16 * TILES];                                 // scale times g^n and n g^(n-1)
+    __shared__ double part_s[2 * TILES];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, lq = lane >> 4;
+    const int64_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
+    const int len = static_cast<int>(sequence_length(a.lengths, b, a.time));
+    const int mine = 16 * (wave >> 1), role = wave & 1;              // first position of the tile; 0: k and dv, 1: v and dk
+    const int pos = mine + l16;
+    const int64_t step_i = a.batch * a.heads * a.di, step_j = a.batch * a.heads * a.dj;
+    const float *q = a.q + bh * a.di, *dout = a.dout + bh * a.dj, *k = a.k + bh * a.di, *v = a.v + bh * a.dj;
+    R q_n, do_n;
+    f4 own[N];
+    if (len > 0) {
+        q_n.fetch(q, step_i, a.di, 0, len);
+        do_n.fetch(dout, step_j, a.dj, 0, len);
+        const int row = pos < len ? pos : len - 1;
+        read_operand(own, role ? v + row * step_j : k + row * step_i, role ? a.dj : a.di, lq);
+    }
+    if (tid < 16 * TILES) {
+        const double g = a.decay[h];
+        pk[tid] = a.scale * static_cast<float>(power(g, tid));
+        sk[tid] = tid ? a.scale * static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
+    }
+    // columns that a row does not have: zeros, which nothing overwrites
+    for (int e = tid * 4; e < 2 * kRows; e += kThreads * 4) {
+        *reinterpret_cast<f4*>(q_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        *reinterpret_cast<f4*>(do_all + e) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    f4 acc[N];
+#pragma unroll
+    for (int it = 0; it < N; ++it) acc[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
+
+    int turn = 0;
+    for (int first = 0; first < len; first += kChunk, turn ^= 1) {
+        float *const q_s = q_all + turn * kRows, *const do_s = do_all + turn * kRows;
+        q_n.put(q_s, a.di, first, len);
+        do_n.put(do_s, a.dj, first, len);
+        __syncthreads();                       // two buffers: nobody reads the ones before the last any more
+        const bool more = first + kChunk < len;
+        q_n.fetch(more ? q : k, step_i, a.di, more ? first + kChunk : 0, len);      // k: for what follows the loop
+        do_n.fetch(dout, step_j, a.dj, first + kChunk, len);
+        for (int x = first; x < first + kChunk; x += 16) {
+            if (x < mine || x >= len) continue;
+            const f4 s = scores<N>((role ? do_s : q_s) + (x - first) * LD, own, l16, lq);
+            float* to = (role ? p_all : s_all) + ((x >> 4) * ((x >> 4) + 1) / 2 + (mine >> 4)) * kTile + 4 * lq * kLD + l16;
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = x + 4 * lq + r, e = row - pos;
+                const bool seen = e >= 0 && row < len;                   // otherwise 0 whatever the score
+                w[r] = seen ? s[r] * pk[e] : 0.0f;
+                to[r * kLD] = seen ? (role ? s[r] : s[r] * sk[e]) : 0.0f;
+            }
+            add_rows<N, LD, true>(acc, w, (role ? q_s : do_s) + (x - first) * LD, x == mine, l16, lq);
+        }
+    }
+    // lane: position pos, columns 16 it + 4 lq .. + 3
+    if (pos < len) {
+        float* to = role ? a.dk + pos * step_i + bh * a.di : a.dv + pos * step_j + bh * a.dj;
+        const int d = role ? a.di : a.dj;
+#pragma unroll
+        for (int it = 0; it < N; ++it) store4(to + 16 * it + 4 * lq, acc[it], d - 16 * it - 4 * lq);
+    }
+
+    f4 dq[kHalf];
+#pragma unroll
+    for (int it = 0; it < kHalf; ++it) dq[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    double slope = 0.0;
+    for (int first = 0; first < len; first += kChunk, turn ^= 1) {
+        float* const k_s = q_all + turn * kRows;
+        q_n.put(k_s, a.di, first, len);
+        __syncthreads();
+        if (first + kChunk < len) q_n.fetch(k, step_i, a.di, first + kChunk, len);
+        for (int x = first; x < first + kChunk; x += 16) {
+            if (x > mine || mine >= len) continue;
+            const int at = ((mine >> 4) * ((mine >> 4) + 1) / 2 + (x >> 4)) * kTile + l16 * kLD + 4 * lq;
+            const f4 p = *reinterpret_cast<const f4*>(p_all + at);
+            if (a.slope && (x >> 4 & 1) == role) {
+                const f4 s = *reinterpret_cast<const f4*>(s_all + at);
+                slope += static_cast<double>((p[0] * s[0] + p[1] * s[1]) + (p[2] * s[2] + p[3] * s[3]));
+            }
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int e = pos - x - 4 * lq - r;
+                w[r] = e >= 0 ? p[r] * pk[e] : 0.0f;
+            }
+            add_rows<kHalf, LD, false>(dq, w, k_s + (x - first) * LD + role * 16 * kHalf, x == mine, l16, lq);
+        }
+    }
+    if (pos < len)
+#pragma unroll
+        for (int it = 0; it < kHalf; ++it) {
+            const int col = 16 * (role * kHalf + it) + 4 * lq;
+            store4(a.dq + pos * step_i + bh * a.di + col, dq[it], a.di - col);
+        }
+    // rows behind the sequence's end
+    for (int64_t x = len + wave; x < a.time; x += 2 * TILES) {
+        for (int i = lane; i < a.di; i += kWave) a.dq[x * step_i + bh * a.di + i] = a.dk[x * step_i + bh * a.di + i] = 0.0f;
+        for (int j = lane; j < a.dj; j += kWave) a.dv[x * step_j + bh * a.dj + j] = 0.0f;
+    }
+    if (a.slope) {
         for (int d = 1; d < kWave; d <<= 1) slope += __shfl_xor(slope, d);
         if (lane == 0) part_s[wave] = slope;
         __syncthreads();
         if (tid == 0) {
             double s = 0.0;
-            for (int x = 0; x < 8; ++x) s += part_s[x];
-            a.slope[blockIdx.x] = s;
+            for (int x = 0; x < 2 * TILES; ++x) s += part_s[x];
+            a.slope[bh] = s;
         }
     }
 }
@@ -934,50 +1063,76 @@ void launch_pass(const Passes& p, int di, int dj, dim3 grid) {
     else launch_pass<8, TAN, STATE>(p, dj, grid);
 }
 
-template <int NI, bool TAN>
-void launch_scores(const Passes& p, int dj, dim3 grid) {
-    if (dj <= 32) hipLaunchKernelGGL((la_scores_kernel<NI, 2, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
-    else if (dj <= 64) hipLaunchKernelGGL((la_scores_kernel<NI, 4, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
-    else hipLaunchKernelGGL((la_scores_kernel<NI, 8, TAN>), grid, dim3(8 * kWave), 0, ctx().stream, p);
+template <int NI>
+void launch_scores(const PassArgs& a, dim3 grid) {
+    if (a.dj <= 32) hipLaunchKernelGGL((la_scores_kernel<NI, 2>), grid, dim3(8 * kWave), 0, ctx().stream, a);
+    else if (a.dj <= 64) hipLaunchKernelGGL((la_scores_kernel<NI, 4>), grid, dim3(8 * kWave), 0, ctx().stream, a);
+    else hipLaunchKernelGGL((la_scores_kernel<NI, 8>), grid, dim3(8 * kWave), 0, ctx().stream, a);
 }
-template <bool TAN>
-void launch_scores(const Passes& p, int di, int dj, dim3 grid) {
-    if (di <= 32) launch_scores<2, TAN>(p, dj, grid);
-    else if (di <= 64) launch_scores<4, TAN>(p, dj, grid);
-    else launch_scores<8, TAN>(p, dj, grid);
+template <int N>
+void launch_scores_bwd(const BackArgs& a, dim3 grid) {
+    if (a.time <= 64) hipLaunchKernelGGL((la_scores_bwd_kernel<N, 4>), grid, dim3(8 * kWave), 0, ctx().stream, a);
+    else hipLaunchKernelGGL((la_scores_bwd_kernel<N, 8>), grid, dim3(16 * kWave), 0, ctx().stream, a);
+}
+
+int check_steps(int64_t sequences, int di, int dj) {
+    if (sequences * (di > dj ? di : dj) > kStepFloats)
+        return set_error(BSHIP_ERR_UNSUPPORTED, "linear attention: more than %lld features in a time step",
+                         static_cast<long long>(kStepFloats));
+    return 0;
+}
+
+// A launch has fewer than 2^32 threads.
+int check_blocks(int64_t blocks, int threads) {
+    if (blocks > 0xffffffffll / threads)
+        return set_error(BSHIP_ERR_BAD_DIMENSION, "linear attention: %lld workgroups exceed one launch",
+                         static_cast<long long>(blocks));
+    return 0;
+}
+
+int sum_slopes(const Scratch& parts, float* ddecay, int64_t batch, int64_t heads, int64_t per_head) {
+    hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(heads)), dim3(kBlock), 0, ctx().stream,
+                       static_cast<const double*>(parts.p), ddecay, batch, heads, per_head);
+    return check_launch("linear attention, decay gradient");
+}
+
+int run_scores(const PassArgs& a) {
+    const int64_t sequences = a.batch * a.heads;
+    int st = check_steps(sequences, a.di, a.dj);
+    if (st != 0 || (st = check_blocks(sequences, 8 * kWave)) != 0) return st;
+    const dim3 grid(static_cast<unsigned>(sequences));
+    if (a.di <= 32) launch_scores<2>(a, grid);
+    else if (a.di <= 64) launch_scores<4>(a, grid);
+    else launch_scores<8>(a, grid);
+    return check_launch("linear attention, all scores");
+}
+
+int run_scores_bwd(BackArgs a, float* ddecay) {
+    const int64_t sequences = a.batch * a.heads;
+    int st = check_steps(sequences, a.di, a.dj);
+    if (st != 0 || (st = check_blocks(sequences, 16 * kWave)) != 0) return st;
+    Scratch slope;
+    if (ddecay && (st = slope.get(sequences * sizeof(double))) != 0) return st;
+    a.slope = static_cast<double*>(slope.p);
+    const int d = a.di > a.dj ? a.di : a.dj;
+    const dim3 grid(static_cast<unsigned>(sequences));
+    if (d <= 32) launch_scores_bwd<2>(a, grid);
+    else if (d <= 64) launch_scores_bwd<4>(a, grid);
+    else launch_scores_bwd<8>(a, grid);
+    st = check_launch("linear attention, gradients from all scores");
+    return st != 0 || !ddecay ? st : sum_slopes(slope, ddecay, a.batch, a.heads, 1);
 }
 
 // `count` passes over the same sequences side by side. ddecay: with the derivative by the decay (one pass).
 int run_passes(Passes p, int count, float* ddecay) {
     const PassArgs& a = p.pass[0];
     const int64_t sequences = a.batch * a.heads;
-    if (sequences * (a.di > a.dj ? a.di : a.dj) > kStepFloats)
-        return set_error(BSHIP_ERR_UNSUPPORTED, "linear attention: more than %lld features in a time step",
-                         static_cast<long long>(kStepFloats));
+    int st = check_steps(sequences, a.di, a.dj);
+    if (st != 0) return st;
     int di = 0, dj = 0;
     for (int n = 0; n < count; ++n) {
         di = p.pass[n].di > di ? p.pass[n].di : di;
         dj = p.pass[n].dj > dj ? p.pass[n].dj : dj;
-    }
-    // all scores where that is the less work, or nearly: 2 T d against 4 d^2 and the scores inside chunks
-    bool whole = a.time <= kAllScores && a.time * (a.di + a.dj) <= 4 * a.di * a.dj + 32 * (a.di + a.dj);
-    for (int n = 0; n < count; ++n)
-        whole = whole && !p.pass[n].init && !p.pass[n].fin && !p.pass[n].dfin && p.pass[n].di >= 4 && p.pass[n].dj >= 4;
-    if (whole) {
-        Scratch slope;
-        if (ddecay) {
-            int st = slope.get(sequences * sizeof(double));
-            if (st != 0) return st;
-            p.pass[0].slope = static_cast<double*>(slope.p);
-        }
-        const dim3 grid(static_cast<unsigned>(sequences), static_cast<unsigned>(count));
-        if (ddecay) launch_scores<true>(p, di, dj, grid);
-        else launch_scores<false>(p, di, dj, grid);
-        int st = check_launch("linear attention, all scores");
-        if (st != 0 || !ddecay) return st;
-        hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(a.heads)), dim3(kBlock), 0, ctx().stream,
-                           static_cast<const double*>(slope.p), ddecay, a.batch, a.heads, int64_t(1));
-        return check_launch("linear attention, decay gradient");
     }
     // eight wavefronts for every compute unit: where there are fewer sequences, the time axis is cut, into segments of
     // 128 positions at least
@@ -989,17 +1144,15 @@ int run_passes(Passes p, int count, float* ddecay) {
     int64_t seg_len = ceil_div(ceil_div(a.time, segs), kChunk) * kChunk;
     if (seg_len < kChunk) seg_len = kChunk;
     segs = a.time > 0 ? ceil_div(a.time, seg_len) : 1;
-    if (sequences * segs > 0x7fffffff)
-        return set_error(BSHIP_ERR_BAD_DIMENSION, "linear attention: %lld sequences of %lld steps exceed one launch",
-                         static_cast<long long>(sequences), static_cast<long long>(a.time));
+    if ((st = check_blocks(sequences * segs, (dj <= 64 ? 4 : 8) * kWave)) != 0) return st;
     const size_t states = static_cast<size_t>(sequences) * segs * a.di * a.dj * (ddecay ? 2 : 1);
     Scratch seg, slope;
     if (segs > 1) {
-        int st = seg.get(states * count * sizeof(float));
+        st = seg.get(states * count * sizeof(float));
         if (st != 0) return st;
     }
     if (ddecay) {
-        int st = slope.get(sequences * segs * sizeof(double));
+        st = slope.get(sequences * segs * sizeof(double));
         if (st != 0) return st;
     }
     for (int n = 0; n < count; ++n) {
@@ -1013,7 +1166,7 @@ int run_passes(Passes p, int count, float* ddecay) {
     if (segs > 1) {
         if (ddecay) launch_pass<true, true>(p, di, dj, grid);
         else launch_pass<false, true>(p, di, dj, grid);
-        int st = check_launch("linear attention, segment states");
+        st = check_launch("linear attention, segment states");
         if (st != 0) return st;
     }
     if (segs > kAddedUp) {
@@ -1021,25 +1174,21 @@ int run_passes(Passes p, int count, float* ddecay) {
         hipLaunchKernelGGL(la_scan_kernel, dim3(static_cast<unsigned>(ceil_div(a.di * a.dj, kBlock)),
                                                 static_cast<unsigned>(rows), static_cast<unsigned>(count)),
                            dim3(kBlock), 0, ctx().stream, p, ddecay ? 1 : 0);
-        int st = check_launch("linear attention, scan");
+        st = check_launch("linear attention, scan");
         if (st != 0) return st;
     }
     if (ddecay) launch_pass<true, false>(p, di, dj, grid);
     else launch_pass<false, false>(p, di, dj, grid);
-    int st = check_launch("linear attention");
-    if (st != 0 || !ddecay) return st;
-    hipLaunchKernelGGL(la_slope_kernel, dim3(static_cast<unsigned>(a.heads)), dim3(kBlock), 0, ctx().stream,
-                       static_cast<const double*>(slope.p), ddecay, a.batch, a.heads, segs);
-    return check_launch("linear attention, decay gradient");
+    st = check_launch("linear attention");
+    return st != 0 || !ddecay ? st : sum_slopes(slope, ddecay, a.batch, a.heads, segs);
 }
 
 int run_steps(PassArgs a) {
     const int64_t sequences = a.batch * a.heads;
     const bool wide = sequences * ceil_div(a.dj, 64) >= ctx().num_cus;
     a.tiles_j = static_cast<int>(ceil_div(a.dj, wide ? 64 : 16));
-    if (sequences * a.tiles_j > 0x7fffffff)
-        return set_error(BSHIP_ERR_BAD_DIMENSION, "linear attention: %lld sequences exceed one launch",
-                         static_cast<long long>(sequences));
+    int st = check_blocks(sequences * a.tiles_j, kBlock);
+    if (st != 0) return st;
     const dim3 grid(static_cast<unsigned>(sequences * a.tiles_j));
     if (wide) hipLaunchKernelGGL((la_step_kernel<16>), grid, dim3(kBlock), 0, ctx().stream, a);
     else hipLaunchKernelGGL((la_step_kernel<4>), grid, dim3(kBlock), 0, ctx().stream, a);
@@ -1052,6 +1201,13 @@ int check_all(const char* fn, const void* const* ptrs, int count) {
         if (reinterpret_cast<uintptr_t>(ptrs[n]) & 3u)
             return set_error(BSHIP_ERR_BAD_POINTER, "%s: an array is not 4-byte aligned", fn);
     }
+    return 0;
+}
+// Arrays that may be NULL.
+int check_given(const char* fn, const void* const* ptrs, int count) {
+    for (int n = 0; n < count; ++n)
+        if (reinterpret_cast<uintptr_t>(ptrs[n]) & 3u)
+            return set_error(BSHIP_ERR_BAD_POINTER, "%s: an array is not 4-byte aligned", fn);
     return 0;
 }
 int check_dims(const char* fn, int64_t time, int64_t batch, int64_t heads, int64_t dk, int64_t dv) {
@@ -1080,6 +1236,8 @@ int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* 
     if (batch * heads == 0) return 0;
     const void* need[] = {q, k, v, out, decay};
     if (time > 0 && (st = check_all(__func__, need, 5)) != 0) return st;
+    const void* given[] = {decay, lengths, state, new_state};
+    if ((st = check_given(__func__, given, 4)) != 0) return st;
     PassArgs a = {};
     a.q = q; a.k = k; a.v = v; a.out = out;
     a.decay = decay; a.lengths = lengths;
@@ -1090,7 +1248,11 @@ int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* 
     a.kv_scale = 1.0f; a.out_scale = scale;
     if (time == 0 && !new_state) return 0;
     BSHIP_REQUIRE_PTR(decay);
-    return time <= kStepMost ? run_steps(a) : run_passes(Passes{{a}}, 1, nullptr);
+    if (time <= kStepMost) return run_steps(a);
+    // all scores where that is the less work, or nearly: 2 T d against 4 d^2 and the scores inside chunks
+    if (time <= kAllScores && !state && !new_state && dk >= 4 && dv >= 4 && time * (dk + dv) <= 4 * dk * dv + 32 * (dk + dv))
+        return run_scores(a);
+    return run_passes(Passes{{a}}, 1, nullptr);
 }
 
 int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* v, const float* decay,
@@ -1105,6 +1267,11 @@ int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* 
     BSHIP_REQUIRE_PTR(decay);
     const void* need[] = {q, k, v, dout, dq, dk_out, dv_out};
     if (time > 0 && (st = check_all(__func__, need, 7)) != 0) return st;
+    const void* given[] = {decay, lengths, state, dnew_state, ddecay, dstate};
+    if ((st = check_given(__func__, given, 6)) != 0) return st;
+    if (time > 0 && time <= kAllScores && !state && !dnew_state && !dstate && dk >= 4 && dv >= 4)
+        return run_scores_bwd(BackArgs{q, k, v, dout, decay, lengths, dq, dk_out, dv_out, nullptr, time, batch, heads,
+                                       static_cast<int>(dk), static_cast<int>(dv), scale}, ddecay);
     PassArgs a = {};
     a.decay = decay; a.lengths = lengths;
     a.time = time; a.batch = batch; a.heads = heads;
