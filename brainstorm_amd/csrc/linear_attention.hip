@@ -38,7 +38,10 @@ constexpr int kChunk = 32;
 constexpr int64_t kStepFloats = int64_t(1) << 25;      // batch * heads * d of a pass: 31 rows within 4 GiB
 constexpr int kAddedUp = 4;       // up to so many segments a pass adds up what the ones before leave by itself; the scan of
                                   // more is a launch of its own (1024 steps, 128 sequences of 128 features: 685 us with, 760 without)
-constexpr int kStepMost = 4;      // sequences of at most this many positions go position by position
+// Sequences of at most this many positions go position by position; from the next on a pass is as fast or faster (with states;
+// positions 3, 4, 5 one by one against a pass: 163, 193, 222 against 168, 170, 170 us for 4096 sequences of 128 features, 7.0, 8.1,
+// 9.0 against 8.5 us for 256 of 64).
+constexpr int kStepMost = 3;
 
 struct PassArgs {
     const float *q, *k, *v;
@@ -1069,10 +1072,12 @@ void launch_scores(const PassArgs& a, dim3 grid) {
     else if (a.dj <= 64) hipLaunchKernelGGL((la_scores_kernel<NI, 4>), grid, dim3(8 * kWave), 0, ctx().stream, a);
     else hipLaunchKernelGGL((la_scores_kernel<NI, 8>), grid, dim3(8 * kWave), 0, ctx().stream, a);
 }
+// 64 steps need half of the wavefronts and a quarter of the tiles: two workgroups share a compute unit up to 64 features (800
+// sequences of 64 steps of 64 features: 40 us, with room for 128 steps 59).
 template <int N>
 void launch_scores_bwd(const BackArgs& a, dim3 grid) {
-    if (a.time <= 64) hipLaunchKernelGGL((la_scores_bwd_kernel<N, 4>), grid, dim3(8 * kWave), 0, ctx().stream, a);
-    else hipLaunchKernelGGL((la_scores_bwd_kernel<N, 8>), grid, dim3(16 * kWave), 0, ctx().stream, a);
+    if (a.time <= kAllScores / 2) hipLaunchKernelGGL((la_scores_bwd_kernel<N, 4>), grid, dim3(8 * kWave), 0, ctx().stream, a);
+    else if constexpr (N > 2) hipLaunchKernelGGL((la_scores_bwd_kernel<N, 8>), grid, dim3(16 * kWave), 0, ctx().stream, a);
 }
 
 int check_steps(int64_t sequences, int di, int dj) {
@@ -1134,11 +1139,16 @@ int run_passes(Passes p, int count, float* ddecay) {
         di = p.pass[n].di > di ? p.pass[n].di : di;
         dj = p.pass[n].dj > dj ? p.pass[n].dj : dj;
     }
-    // eight wavefronts for every compute unit: where there are fewer sequences, the time axis is cut, into segments of
-    // 128 positions at least
+    // Eight wavefronts for every compute unit (4, 8 and 16 of them: 206, 175 and 189 us forwards for 128 sequences of 1024 steps
+    // of 128 features, 87, 78 and 93 for 16 of 8192 steps of 64): where there are fewer sequences, the time axis is cut, into
+    // segments of 64 positions at least (37 us, with 128 positions 48, for 15 sequences of 777 steps of 72 features; 32
+    // positions save nothing there and cost 10 % elsewhere). More than the scan loads at once, only of 128 (8 sequences of
+    // 4000 steps of 64 features: 44 us, with 64 positions 54).
     int64_t want = 8 * static_cast<int64_t>(ctx().num_cus) / (dj <= 64 ? 4 : 8);
     int64_t segs = ceil_div(want, sequences * count);
-    const int64_t most = ceil_div(a.time, 4 * kChunk);
+    int64_t most = ceil_div(a.time, 2 * kChunk);
+    if (most > kScanned) most = kScanned;
+    if (most < ceil_div(a.time, 4 * kChunk)) most = ceil_div(a.time, 4 * kChunk);
     if (segs > most) segs = most;
     if (segs < 1) segs = 1;
     int64_t seg_len = ceil_div(ceil_div(a.time, segs), kChunk) * kChunk;
@@ -1185,7 +1195,9 @@ int run_passes(Passes p, int count, float* ddecay) {
 
 int run_steps(PassArgs a) {
     const int64_t sequences = a.batch * a.heads;
-    const bool wide = sequences * ceil_div(a.dj, 64) >= ctx().num_cus;
+    // 64 columns for a workgroup where that still makes many of them, 16 otherwise (one step, heads of 64 features: 16.2 against
+    // 18.0 us for 2048 sequences, 6.4 against 6.1 for 512; 112 us for 4096 sequences of 128 features)
+    const bool wide = sequences * ceil_div(a.dj, 64) >= 4 * static_cast<int64_t>(ctx().num_cus);
     a.tiles_j = static_cast<int>(ceil_div(a.dj, wide ? 64 : 16));
     int st = check_blocks(sequences * a.tiles_j, kBlock);
     if (st != 0) return st;
@@ -1249,8 +1261,10 @@ int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* 
     if (time == 0 && !new_state) return 0;
     BSHIP_REQUIRE_PTR(decay);
     if (time <= kStepMost) return run_steps(a);
-    // all scores where that is the less work, or nearly: 2 T d against 4 d^2 and the scores inside chunks
-    if (time <= kAllScores && !state && !new_state && dk >= 4 && dv >= 4 && time * (dk + dv) <= 4 * dk * dv + 32 * (dk + dv))
+    // all scores where that is less work than a state: up to 1.5 d steps (800 sequences, chunks against scores: 64 features, 64, 96
+    // and 128 steps, 22.4, 30.0, 37.4 against 19.6, 29.8, 42.0 us; 32 features, 32 and 64 steps, 8.2, 11.7 against 8.1, 12.6;
+    // 125 features, 128 steps, 103 against 75)
+    if (time <= kAllScores && !state && !new_state && dk >= 4 && dv >= 4 && time * (dk + dv) <= 3 * dk * dv)
         return run_scores(a);
     return run_passes(Passes{{a}}, 1, nullptr);
 }
@@ -1269,7 +1283,11 @@ int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* 
     if (time > 0 && (st = check_all(__func__, need, 7)) != 0) return st;
     const void* given[] = {decay, lengths, state, dnew_state, ddecay, dstate};
     if ((st = check_given(__func__, given, 6)) != 0) return st;
-    if (time > 0 && time <= kAllScores && !state && !dnew_state && !dstate && dk >= 4 && dv >= 4)
+    // The gradients take more passes, so that all scores win up to 64 steps whatever the features (800 sequences of 16: 28.8
+    // against 31.0 us) and up to 128 with more than 32 (64 and 125 features: 117 against 124, 196 against 392 us; 32: 84
+    // against 61).
+    if (time > 0 && time <= (dk > 32 || dv > 32 ? kAllScores : kAllScores / 2) && !state && !dnew_state && !dstate && dk >= 4 &&
+        dv >= 4)
         return run_scores_bwd(BackArgs{q, k, v, dout, decay, lengths, dq, dk_out, dv_out, nullptr, time, batch, heads,
                                        static_cast<int>(dk), static_cast<int>(dv), scale}, ddecay);
     PassArgs a = {};

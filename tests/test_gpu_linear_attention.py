@@ -12,6 +12,7 @@ import threading
 import numpy as np
 import pytest
 
+from brainstorm_amd import _lib
 from oracle import sequence_ops as ops
 from util import assert_bit_equal
 
@@ -244,10 +245,14 @@ def test_arrays_that_start_anywhere(hip, shift):
     want, want_new = forward(hip, a, True)
     want_back = backward(hip, a, True)
 
+    whole = []
+
     def up(x):
         flat = hip.zeros((x.size + 8,))
+        hip.fill(flat, 3.0)
         view = flat[shift:shift + x.size].reshape(x.shape)
         hip.set_from_numpy(view, x)
+        whole.append((flat, x.size))
         return view
 
     q, k, v, decay, state, dout, dnew = (up(a[n]) for n in ("q", "k", "v", "decay", "state", "dout", "dnew"))
@@ -259,9 +264,9 @@ def test_arrays_that_start_anywhere(hip, shift):
     assert_bit_equal(new.get(), want_new)
     for x, w in zip((dq, dk, dv, ddecay, dstate), want_back):
         assert_bit_equal(x.get(), w)
-    for x in (out, new, dq, dk, dv, ddecay, dstate):               # nothing around the arrays was written
-        flat = x.reshape((x.size,))
-        del flat
+    for flat, size in whole:                                       # nothing around the arrays was written
+        around = flat.get()
+        assert (around[:shift] == 3).all() and (around[shift + size:] == 3).all()
 
 
 def test_the_same_bits_every_time_and_in_a_recording(hip):
@@ -326,3 +331,149 @@ def test_row_pitched_views(hip):
     assert not got[:, :, :3].any() and not got[:, :, 19:].any()
     assert_bit_equal(state.get(), want_new)
     hip.set_fusing(True)
+
+
+# Short sequences without states, where all scores are formed: every width of the kernels, both lengths of the gradients',
+# and sizes on both sides of the rules that choose them.
+SHORT = [(5, 3, 2, 4, 4), (16, 2, 3, 30, 32), (17, 2, 2, 24, 60), (33, 2, 2, 31, 100), (48, 2, 2, 64, 20), (64, 3, 1, 50, 64),
+         (64, 2, 2, 36, 125), (63, 2, 2, 128, 31), (65, 2, 2, 100, 33), (90, 2, 2, 33, 60), (96, 2, 2, 64, 64),
+         (97, 2, 2, 60, 64), (100, 2, 2, 24, 20), (112, 2, 1, 127, 126), (128, 2, 2, 128, 128), (128, 3, 2, 40, 7),
+         (129, 2, 1, 128, 128)]
+
+
+@pytest.mark.parametrize("shape", SHORT)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_short_sequences_without_states(hip, shape, ragged):
+    a = inputs(sum(shape) + 30, *shape, ragged=ragged)
+    check_forward(hip, a, False)
+    check_backward(hip, a, False)
+
+
+def test_many_short_sequences(hip):
+    a = inputs(31, 9, 700, 3, 12, 16, ragged=True)
+    check_forward(hip, a, False)
+    check_backward(hip, a, False)
+
+
+@pytest.mark.parametrize("decay", [[0.0, 1.0], [-0.5, 1.01], [1e-20, 0.999]])
+def test_decays_at_the_ends_without_states(hip, decay):
+    a = inputs(32, 70, 2, 2, 40, 48, ragged=True)
+    a["decay"] = np.array(decay, F32)
+    check_forward(hip, a, False)
+    check_backward(hip, a, False)
+
+
+@pytest.mark.parametrize("time,at", [(40, 5), (100, 20), (128, 99)])
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+def test_values_that_are_not_finite_without_states(hip, time, at, name):
+    a = inputs(33, time, 2, 2, 120, 124)
+    clean, _ = forward(hip, a, False)
+    a[name][at, 0, 3] = np.nan
+    a[name][at + 1, 0, 5] = np.inf
+    out, _ = forward(hip, a, False)
+    first, second = (slice(0, 124), slice(124, 248))
+    assert_bit_equal(out[:at], clean[:at])
+    assert_bit_equal(out[:, 1], clean[:, 1])
+    assert_bit_equal(out[:, 0, second], clean[:, 0, second])
+    assert not np.isfinite(out[at, 0, first]).all()
+    if name == "q":                                                      # a query is its own position's alone
+        assert_bit_equal(out[at + 2:], clean[at + 2:])
+    if name == "v":                                                      # and a value its own column's
+        rest = np.ones(248, bool)
+        rest[[3, 5]] = False
+        assert_bit_equal(out[:, :, rest], clean[:, :, rest])
+        assert np.isnan(out[at:, 0, 3]).all() and not np.isfinite(out[at + 1:, 0, 5]).any()
+
+
+@pytest.mark.parametrize("time,at,d", [(40, 5, 16), (64, 33, 60), (100, 50, 128), (128, 99, 40)])
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+def test_gradients_that_are_not_finite_without_states(hip, time, at, d, name):
+    a = inputs(34, time, 1, 2, d, d)
+    clean = backward(hip, a, False)
+    a[name][at, 0, 3] = np.nan
+    got = backward(hip, a, False)
+    for n in range(3):                                                   # the other head
+        assert_bit_equal(got[n][:, :, d:], clean[n][:, :, d:])
+    if name in ("q", "dout"):                                            # seen by itself and the keys up to it
+        assert_bit_equal(got[0][:at], clean[0][:at])
+        assert_bit_equal(got[0][at + 1:], clean[0][at + 1:])
+        for n in (1, 2):
+            assert_bit_equal(got[n][at + 1:], clean[n][at + 1:])
+        assert not np.isfinite(got[1][at]).all() and not np.isfinite(got[2][at]).all()
+    else:                                                                # by itself and the queries from it on
+        assert_bit_equal(got[0][:at], clean[0][:at])
+        assert not np.isfinite(got[0][at]).all()
+        for n in (1, 2):
+            assert_bit_equal(got[n][:at], clean[n][:at])
+            assert_bit_equal(got[n][at + 1:], clean[n][at + 1:])
+
+
+@pytest.mark.parametrize("time", [20, 100])
+def test_padding_without_states(hip, time):
+    a = inputs(35, time, 4, 2, 36, 40)
+    a["lengths"] = np.array([time, 0, time // 2 + 0.9, np.nan], F32)
+    lengths = ops.sequence_lengths(a["lengths"], time, 4)
+    clean_out, _ = forward(hip, a, False)
+    clean = backward(hip, a, False)
+    for b, n in enumerate(lengths):
+        for name in ("q", "k", "v", "dout"):
+            a[name][n:, b] = np.nan if b % 2 else np.inf
+    assert_bit_equal(forward(hip, a, False)[0], clean_out)
+    for x, y in zip(backward(hip, a, False)[:4], clean):
+        assert_bit_equal(x, y)
+    for b, n in enumerate(lengths):
+        for x in (clean_out, clean[0], clean[1], clean[2]):
+            assert not x[n:, b].any()
+
+
+@pytest.mark.parametrize("shape", [(30, 2, 2, 21, 23), (100, 2, 2, 125, 125)])
+def test_short_sequences_anywhere_and_recorded(hip, shape):
+    a = inputs(36, *shape)
+    want_out, _ = forward(hip, a, False)
+    want = [want_out] + backward(hip, a, False)[:4]
+    whole = []
+
+    def up(x, shift):
+        flat = hip.zeros((x.size + 8,))
+        hip.fill(flat, 3.0)
+        hip.set_from_numpy(flat[shift:shift + x.size].reshape(x.shape), x)
+        whole.append((flat, shift, x.size))
+        return flat[shift:shift + x.size].reshape(x.shape)
+
+    q, k, v, dout, decay = (up(a[n], 1 + i % 3) for i, n in enumerate(("q", "k", "v", "dout", "decay")))
+    results = [up(np.ones_like(w), 3 - i % 3) for i, w in enumerate(want)]
+
+    def run():
+        hip.linear_attention_forward(q, k, v, decay, results[0], 0.3)
+        hip.linear_attention_backward(q, k, v, decay, dout, *results[1:], scale=0.3)
+
+    run()
+    first, second = hip.record(run), hip.record(run)
+    for step in (None, first, second, first):
+        if step is not None:
+            for x in results:
+                hip.fill(x, 7.0)
+            step.replay()
+        for x, w in zip(results, want):
+            assert_bit_equal(x.get(), w)
+        run()
+        for flat, shift, size in whole:
+            around = flat.get()
+            assert (around[:shift] == 3).all() and (around[shift + size:] == 3).all()
+    first.release()
+    second.release()
+
+
+def test_more_features_than_a_pass_reaches(hip):
+    # 2^25 + 1024 features in a step: refused for 4 steps, computed position by position for 3
+    batch = 2 ** 15 + 1
+    x, out = hip.zeros((4, batch, 1024)), hip.ones((4, batch, 1024))
+    decay = hip.ones((8,))
+    with pytest.raises(_lib.BshipError, match="features in a time step"):
+        hip.linear_attention_forward(x, x, x, decay, out)
+    assert (out[3][batch - 1].get() == 1).all()
+    hip.fill(x, 1.0)
+    hip.linear_attention_forward(x[:3], x[:3], x[:3], decay, out[:3])
+    for t in range(3):
+        for b in (0, batch - 1):
+            assert_bit_equal(out[t][b].get(), np.full(1024, 128.0 * (t + 1), F32))
