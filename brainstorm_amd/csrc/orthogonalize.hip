@@ -16,6 +16,11 @@
 //
 // A and p are symmetric: only the tiles on and above the diagonal are computed and each is written twice. X is kept
 // in both orientations, so every product has both operands contiguous along the summed axis.
+//
+// The float16 matrix rate bounds large matrices (a large product reaches 1349 TFLOP/s, three of them for each of ours):
+// the momentum update of 4096 x 4096 takes 3.59 ms, of which products that cannot be left out 3.05; 4 x 1000 x 1000 take
+// 0.42 ms (0.18): rounds of tiles that do not fill the card; 1200 x 784 takes 0.18 ms (0.03): 17 launches of 10 to 13 us, each
+// a chain of its steps' waits.
 #include "common.h"
 
 #pragma clang fp contract(off)
