@@ -30,10 +30,10 @@
 //
 // What bounds it and what it takes (a large copy moves 5.1 TB/s on this card, a float32 product reaches 152 TFLOP/s):
 //   one step, 4096 sequences of 128 x 128: the state in and out, 537 MB: 106 us, 5.1 TB/s; 8 sequences: a launch, 3.7 us
-//   16 sequences of 8192 steps of 64: 72 us in three launches (states of the segments 22, scan 6, pass 45); 134 MB would
+//   16 sequences of 8192 steps of 64: 70 us in three launches (states of the segments 22, scan 6, pass 45); 134 MB would
 //     take 26 us, but a segment's chunks wait for each other
-//   128 sequences of 1024 steps of 128: forward 168 us, backward 495; 30 GFLOP that cannot be left out take 198 us; 60 % of
-//     the matrix rate inside a pass, the rest is the states of segments and the derivative by the decay, a fifth each
+//   128 sequences of 1024 steps of 128: forward 153 us, backward 464; 30 GFLOP that cannot be left out take 198 us; 60 % of
+//     the matrix rate inside a pass, the rest is the derivative by the decay, a quarter of the work
 //   800 sequences of 100 steps of 125, all scores: forward 66 us, backward 168 us
 #include "common.h"
 
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
     const int64_t pe = len < p1 ? (len > p0 ? len : p0) : p1;      // valid positions [p0, pe)
     const double g = a.decay[h];
     const float gf = a.decay[h];
-    const int j0 = 16 * wave;                                      // this wavefront's columns
+    const int j0 = 16 * (NW * static_cast<int>(blockIdx.z) + wave);       // this wavefront's columns
     const bool mine = j0 < a.dj;
 
     // Position p is time p forwards, len - 1 - p backwards. Rows are addressed from a chunk's earliest time, which is
@@ -566,7 +566,8 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
     }
     // rows behind the sequence's end: there position p is time p in both directions
     for (int64_t p = (len > p0 ? len : p0) + wave; p < p1; p += NW)
-        for (int j = lane; j < a.dj; j += kWave) a.out[(p * a.batch * a.heads + bh) * a.dj + j] = 0.0f;
+        for (int j = 16 * NW * static_cast<int>(blockIdx.z) + lane; j < a.dj && j < 16 * NW * static_cast<int>(blockIdx.z + 1); j += kWave)
+            a.out[(p * a.batch * a.heads + bh) * a.dj + j] = 0.0f;
     // the workgroup of the segment with the last position has the final state
     const bool last = len > 0 ? (pe == len && pe > p0) : seg == 0;
     if (last && (a.fin || (TAN && a.dfin))) {
@@ -588,7 +589,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
         if (tid == 0) {
             double s = 0.0;
             for (int x = 0; x < NW; ++x) s += part_s[x];
-            a.slope[blockIdx.x] = s;
+            a.slope[blockIdx.x * gridDim.z + blockIdx.z] = s;
         }
     }
 }
@@ -1066,7 +1067,7 @@ struct Scratch {
 
 template <int NI, bool TAN, bool STATE, bool NARROW = false>
 void launch_pass(const Passes& p, int dj, dim3 grid) {
-    if (dj <= 64) hipLaunchKernelGGL((la_pass_kernel<NI, 4, TAN, STATE, NARROW>), grid, dim3(4 * kWave), 0, ctx().stream, p);
+    if (dj <= 64 * static_cast<int>(grid.z)) hipLaunchKernelGGL((la_pass_kernel<NI, 4, TAN, STATE, NARROW>), grid, dim3(4 * kWave), 0, ctx().stream, p);
     else hipLaunchKernelGGL((la_pass_kernel<NI, 8, TAN, STATE, NARROW>), grid, dim3(8 * kWave), 0, ctx().stream, p);
 }
 template <bool TAN, bool STATE>
@@ -1151,22 +1152,31 @@ int run_passes(Passes p, int count, float* ddecay) {
         di = p.pass[n].di > di ? p.pass[n].di : di;
         dj = p.pass[n].dj > dj ? p.pass[n].dj : dj;
     }
-    // Eight wavefronts for every compute unit (4, 8 and 16 of them: 206, 175 and 189 us forwards for 128 sequences of 1024 steps
+    // Eight wavefronts for every compute unit (4, 8 and 16 of them: 94, 65 and 74 us forwards for 16 sequences of 2048 steps
     // of 128 features, 87, 78 and 93 for 16 of 8192 steps of 64): where there are fewer sequences, the time axis is cut, into
     // segments of 64 positions at least (37 us, with 128 positions 48, for 15 sequences of 777 steps of 72 features; 32
     // positions save nothing there and cost 10 % elsewhere). More than the scan loads at once, only of 128 (8 sequences of
     // 4000 steps of 64 features: 44 us, with 64 positions 54).
-    int64_t want = 8 * static_cast<int64_t>(ctx().num_cus) / (dj <= 64 ? 4 : 8);
-    int64_t segs = ceil_div(want, sequences * count);
+    const int64_t cus = ctx().num_cus, workgroups = sequences * count;
+    int64_t segs = ceil_div(cus * (dj <= 64 ? 2 : 1), workgroups), parts = 1;
     int64_t most = ceil_div(a.time, 2 * kChunk);
     if (most > kScanned) most = kScanned;
     if (most < ceil_div(a.time, 4 * kChunk)) most = ceil_div(a.time, 4 * kChunk);
     if (segs > most) segs = most;
     if (segs < 1) segs = 1;
+    if (dj > 64) {
+        // Two workgroups with half of the columns each, instead of two segments, of which the second waits for the first's
+        // state (1024 steps, 128 and 192 sequences of 128 features: 153 and 231 us forwards, with segments 175 and 297), and
+        // where the time axis cannot be cut further (4 sequences of 300 steps: 30 us, whole 36).
+        if (segs == 2) parts = 2, segs = 1;
+        else if (2 * workgroups * segs <= cus) parts = 2;
+    } else if (4 * workgroups >= 5 * cus) {
+        segs = 1;      // (64 features, 320 and 448 sequences of 1024 steps: 142 and 146 us, with two segments 146 and 184; 160: 106, 84)
+    }
     int64_t seg_len = ceil_div(ceil_div(a.time, segs), kChunk) * kChunk;
     if (seg_len < kChunk) seg_len = kChunk;
     segs = a.time > 0 ? ceil_div(a.time, seg_len) : 1;
-    if ((st = check_blocks(sequences * segs, (dj <= 64 ? 4 : 8) * kWave)) != 0) return st;
+    if ((st = check_blocks(sequences * segs, 8 * kWave)) != 0) return st;
     const size_t states = static_cast<size_t>(sequences) * segs * a.di * a.dj * (ddecay ? 2 : 1);
     Scratch seg, slope;
     if (segs > 1) {
@@ -1174,7 +1184,7 @@ int run_passes(Passes p, int count, float* ddecay) {
         if (st != 0) return st;
     }
     if (ddecay) {
-        st = slope.get(sequences * segs * sizeof(double));
+        st = slope.get(sequences * segs * parts * sizeof(double));
         if (st != 0) return st;
     }
     for (int n = 0; n < count; ++n) {
@@ -1184,7 +1194,7 @@ int run_passes(Passes p, int count, float* ddecay) {
         p.pass[n].seg = segs > 1 ? static_cast<float*>(seg.p) + n * states : nullptr;
         p.pass[n].slope = static_cast<double*>(slope.p);
     }
-    const dim3 grid(static_cast<unsigned>(sequences * segs), static_cast<unsigned>(count));
+    const dim3 grid(static_cast<unsigned>(sequences * segs), static_cast<unsigned>(count), static_cast<unsigned>(parts));
     if (segs > 1) {
         if (ddecay) launch_pass<true, true>(p, di, dj, grid);
         else launch_pass<false, true>(p, di, dj, grid);
@@ -1203,7 +1213,7 @@ int run_passes(Passes p, int count, float* ddecay) {
     if (ddecay) launch_pass<true, false>(p, di, dj, grid);
     else launch_pass<false, false>(p, di, dj, grid);
     st = check_launch("linear attention");
-    return st != 0 || !ddecay ? st : sum_slopes(slope, ddecay, a.batch, a.heads, segs);
+    return st != 0 || !ddecay ? st : sum_slopes(slope, ddecay, a.batch, a.heads, segs * parts);
 }
 
 int run_steps(PassArgs a) {

@@ -477,3 +477,14 @@ def test_more_features_than_a_pass_reaches(hip):
     for t in range(3):
         for b in (0, batch - 1):
             assert_bit_equal(out[t][b].get(), np.full(1024, 128.0 * (t + 1), F32))
+
+
+# Longer sequences by their number: columns in two parts (half of the compute units' number of sequences, or too few positions
+# to cut), segments, neither.
+@pytest.mark.parametrize("shape", [(200, 16, 8, 16, 80), (150, 33, 4, 20, 128), (300, 2, 2, 128, 100), (140, 40, 8, 8, 16),
+                                   (700, 9, 8, 24, 72), (160, 64, 4, 12, 70)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_numbers_of_sequences(hip, shape, ragged):
+    a = inputs(sum(shape) + 40, *shape, ragged=ragged)
+    check_forward(hip, a, True)
+    check_backward(hip, a, True)
