@@ -44,8 +44,10 @@ namespace {
 
 constexpr int kChunk = 32;
 constexpr int64_t kStepFloats = int64_t(1) << 25;      // batch * heads * d of a pass: 31 rows within 4 GiB
-constexpr int kAddedUp = 4;       // up to so many segments a pass adds up what the ones before leave by itself; the scan of
-                                  // more is a launch of its own (1024 steps, 128 sequences of 128 features: 685 us with, 760 without)
+// Up to so many segments a pass adds up what the ones before leave by itself; the scan of more is a launch of its own (1024
+// steps, 160 sequences of 64 features, 4 segments: 83 us forwards, with the scan 90; 64 sequences, 8 segments: 47 and 44; 64
+// sequences of 128 features, 4 segments: 116 and 106 forwards, 304 and 314 backwards).
+constexpr int kAddedUp = 4;
 // Sequences of at most this many positions go position by position; from the next on a pass is as fast or faster (with states;
 // positions 3, 4, 5 one by one against a pass: 163, 193, 222 against 168, 170, 170 us for 4096 sequences of 128 features, 7.0, 8.1,
 // 9.0 against 8.5 us for 256 of 64).
@@ -1187,10 +1189,13 @@ int run_passes(Passes p, int count, float* ddecay) {
         st = slope.get(sequences * segs * parts * sizeof(double));
         if (st != 0) return st;
     }
+    // A state that is replaced has been read by all segments before the last one writes it only if the scan has read it.
+    bool scanned = segs > kAddedUp;
+    for (int n = 0; n < count; ++n) scanned = scanned || (segs > 1 && p.pass[n].init && p.pass[n].init == p.pass[n].fin);
     for (int n = 0; n < count; ++n) {
         p.pass[n].segs = static_cast<int>(segs);
         p.pass[n].seg_len = static_cast<int>(seg_len);
-        p.pass[n].scanned = segs > kAddedUp;
+        p.pass[n].scanned = scanned;
         p.pass[n].seg = segs > 1 ? static_cast<float*>(seg.p) + n * states : nullptr;
         p.pass[n].slope = static_cast<double*>(slope.p);
     }
@@ -1201,7 +1206,7 @@ int run_passes(Passes p, int count, float* ddecay) {
         st = check_launch("linear attention, segment states");
         if (st != 0) return st;
     }
-    if (segs > kAddedUp) {
+    if (scanned) {
         const int64_t rows = sequences < 32768 ? sequences : 32768;
         const dim3 elements(static_cast<unsigned>(ceil_div(a.di * a.dj, kBlock)), static_cast<unsigned>(rows),
                           static_cast<unsigned>(count));

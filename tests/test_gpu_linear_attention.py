@@ -488,3 +488,24 @@ def test_numbers_of_sequences(hip, shape, ragged):
     a = inputs(sum(shape) + 40, *shape, ragged=ragged)
     check_forward(hip, a, True)
     check_backward(hip, a, True)
+
+
+@pytest.mark.parametrize("shape", [(100, 3, 2, 20, 24), (150, 10, 8, 64, 64), (300, 9, 8, 16, 128), (700, 2, 2, 33, 70)])
+def test_a_state_replaced_by_several_segments(hip, shape):
+    # 2 to 11 segments; every one of them starts from the state that the last one replaces
+    a = inputs(sum(shape) + 50, *shape)
+    up = {n: (None if x is None else hip.create_from_numpy(x)) for n, x in a.items()}
+    out, grads = hip.ones(a["v"].shape), [hip.ones(a[n].shape) for n in ("q", "k", "v")]
+    hip.linear_attention_backward(up["q"], up["k"], up["v"], up["decay"], up["dout"], *grads, scale=0.3, state=up["state"],
+                                  dnew_state=up["dnew"], dstate=up["dnew"])
+    hip.linear_attention_forward(up["q"], up["k"], up["v"], up["decay"], out, 0.3, up["state"], up["state"])
+    time, dk, dv = shape[0], shape[3], shape[4]
+    m = {n: np.abs(a[n]) for n in ("q", "k", "v", "decay", "dout", "state", "dnew")}
+    want, size = (ops.linear_attention(x["q"], x["k"], x["v"], x["decay"], 0.3, x["state"]) for x in (a, m))
+    for x, w, s, name in zip((out, up["state"]), want, size, ("out", "new_state")):
+        close(x.get(), w, s, roundings(time, dk), name)
+    want, size = (ops.linear_attention_gradients(x["q"], x["k"], x["v"], x["decay"], x["dout"], 0.3, x["state"], x["dnew"])
+                  for x in (a, m))
+    for n, (x, name) in enumerate(zip(grads + [up["dnew"]], ("dq", "dk", "dv", "dstate"))):
+        n = 4 if name == "dstate" else n
+        close(x.get(), want[n], size[n], roundings(time, max(dk, dv)), name)
