@@ -420,14 +420,14 @@ template <int MODE>
 int launch_product(ProductArgs a, unsigned count) {
     const int64_t cus = ctx().num_cus;
     constexpr int kTiles[] = {256, 192, 128, 64}, kCost[] = {260, 160, 83, 30};
-    int best = 0;
+    int best = 0;                       // (a launch has fewer than 2^32 threads: up to 512 of them for a tile)
     double least = 0.0;
     for (int n = 0; n < 4; ++n) {
         const int64_t side = ceil_div(a.used_p, kTiles[n]), other = ceil_div(a.used_q, kTiles[n]);
         const int64_t tiles = MODE == kGram || MODE == kPoly ? side * (side + 1) / 2 : side * other;
         const int64_t all = tiles * count;
         const double rounds = kTiles[n] == 64 ? static_cast<double>(all > cus ? all : cus) / cus : static_cast<double>(ceil_div(all, cus));
-        if (all > 0x7fffffff || (best && rounds * kCost[n] >= least)) continue;
+        if (all > 0x7fffff || (best && rounds * kCost[n] >= least)) continue;
         least = rounds * kCost[n];
         best = kTiles[n];
         a.tiles_p = static_cast<int>(side);

@@ -1,6 +1,7 @@
 """Shared fixtures. Tests marked ``gpu`` need an MI355X and a built libbship.so;
 everything else runs on the CPU."""
 import ctypes
+import gc
 import os
 import subprocess
 import sys
@@ -15,6 +16,13 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def earlier_garbage():
+    """Collects what the tests of other files left in cycles. A collection in the middle of a test frees their arrays, and
+    a free between two calls ends a sequence of the fusing window, whose launches some tests count."""
+    gc.collect()
 
 
 @pytest.fixture(scope="session")
