@@ -276,8 +276,10 @@ static int flush_deferred_locked() {
     const int count = g_deferred_fill_count.load();
     for (int k = 0; k < count; ++k) most = g_deferred.f[k].n > most ? g_deferred.f[k].n : most;
     const dim3 grid(static_cast<unsigned>((most + kCopyTile - 1) / kCopyTile), static_cast<unsigned>(count));
-    g_deferred_fill_count = 0;
     hipLaunchKernelGGL(multi_fill_kernel, grid, dim3(kBlock), 0, ctx().stream, g_deferred);
+    // Only now: other threads look at the count without the lock, and one that saw 0 before the fills are enqueued would
+    // enqueue ahead of its own.
+    g_deferred_fill_count = 0;
     return check_launch("multi_fill_kernel");
 }
 
