@@ -725,13 +725,22 @@ class GatedResidual(Layer):
                                             epsilon=self.epsilon)
 
     def backward_pass(self, buffers):
+        _h = self.handler
         block, gate = (flatten_time_and_features(buffers.inputs[n]) for n in ("block", "gate"))
-        dblock, dgate, dx = (flatten_time_and_features(buffers.input_deltas[n]) for n in ("block", "gate", "x"))
+        sources = [buffers.input_deltas[n] for n in ("block", "gate", "x")]
+        deltas = [flatten_time_and_features(d) for d in sources]
+        shared = [n for n in (1, 2) if any(sources[n] is d for d in sources[:n])]     # two inputs from one output
+        for n in shared:
+            deltas[n] = _h.zeros(deltas[n].shape)
+        dblock, dgate, dx = deltas
         dh, dy = (flatten_time_and_features(buffers.output_deltas[n]) for n in ("default", "residual"))
-        self.handler.gated_residual_backward(
+        _h.gated_residual_backward(
             self.activation, block, gate, buffers.parameters["post"], buffers.parameters["pre"],
             flatten_time_and_features(buffers.outputs["residual"]), dy, dh, dblock, dgate, dx,
             buffers.gradients["post"], buffers.gradients["pre"], residual_scale=self.residual_scale, epsilon=self.epsilon)
+        for n in shared:
+            d = flatten_time_and_features(sources[n])
+            _h.add_tt(deltas[n], d, out=d)
 
 
 class LinearAttention(Layer):

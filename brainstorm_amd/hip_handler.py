@@ -1472,9 +1472,11 @@ class HipHandler(Handler):
         norms behind a block and before the next one with the block's gate, in one pass. Matrices are
         (rows, width), weights have width elements, rms(v) = sqrt(mean(v * v) + epsilon) over a row. gate may
         be None (no gate), pre_weight and h together (no norm behind). Activations: those of act_func and
-        'swish'."""
+        'swish'. An output may be an input, but y and h are two arrays."""
         code = self._gate_code("gated_residual_forward", activation)
         self._gate_shapes("gated_residual_forward", (block, x, y), (gate,), (post_weight,), pre_weight, (h,))
+        if pre_weight is not None:
+            self._no_overlap("gated_residual_forward", [y, h], ())
         rows, width = x.shape
         self._call(self._lib.bship_gated_residual_fwd_f32(
             code, block.ptr, self._ptr(gate), x.ptr, post_weight.ptr, self._ptr(pre_weight),
@@ -1484,13 +1486,15 @@ class HipHandler(Handler):
                                 dpost_weight, dpre_weight, residual_scale=1.0, epsilon=1e-6, accumulate=True):
         """The gradients of gated_residual_forward. dblock, dgate and dx are added to what they hold (as a layer
         adds to its input deltas) or, with accumulate=False, overwritten; the weights' gradients are
-        overwritten. gate and dgate are None together, and so are pre_weight, dh and dpre_weight."""
+        overwritten. gate and dgate are None together, and so are pre_weight, dh and dpre_weight. No output may be
+        another one: a block's source that is also the gate's needs an array for each."""
         op = "gated_residual_backward"
         code = self._gate_code(op, activation)
         self._gate_shapes(op, (block, dy, dblock, dx), (gate, dgate), (post_weight, dpost_weight), pre_weight,
                           (y, dh), (dpre_weight,))
         if (gate is None) != (dgate is None):
             raise ValueError("%s: gate and dgate go together" % op)
+        self._no_overlap(op, [dblock, dgate, dx, dpost_weight, dpre_weight if pre_weight is not None else None], ())
         rows, width = dx.shape
         self._call(self._lib.bship_gated_residual_bwd_f32(
             code, block.ptr, self._ptr(gate), post_weight.ptr, self._ptr(pre_weight),
@@ -1527,6 +1531,7 @@ class HipHandler(Handler):
         """The gradients of rms_norm_forward; dx is added to what it holds or, with accumulate=False, overwritten,
         dweight is overwritten."""
         self._gate_shapes("rms_norm_backward", (x, dout, dx), (), (weight, dweight), None, ())
+        self._no_overlap("rms_norm_backward", [dx, dweight], ())
         rows, width = x.shape
         self._call(self._lib.bship_gated_residual_bwd_f32(3, None, None, None, weight.ptr, x.ptr, None, dout.ptr, None,
                                                           None, dx.ptr, None, dweight.ptr, rows, width, 1.0, epsilon,

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 from brainstorm_amd.drivers import configs
-from brainstorm_amd.drivers.net import MomentumStepper, OrthogonalStepper
+from brainstorm_amd.drivers.layers import FullyConnected, GatedResidual, Input, Loss, SoftmaxCE
+from brainstorm_amd.drivers.net import MomentumStepper, Net, OrthogonalStepper
 from oracle.sequence_ops import SequenceRefHandler
 
 F32 = np.float32
@@ -46,6 +47,54 @@ def test_backward_pass_adds_to_input_deltas():
         net.layers[name].backward_pass(net.buffers[name])
         assert any(not np.array_equal(d, before[n]) for n, d in net.buffers[name].input_deltas.items()), name
     assert not np.array_equal(net.get("embed", "output_deltas", "default"), once)
+
+
+def shared_sources(handler, fused):
+    """A network whose GatedResidual layers take two and three of their inputs from one output."""
+    layers = [("Input", Input({"default": (9,), "targets": (1,)}), {}),
+              ("embed", FullyConnected(12, "tanh", fused=fused), {"default": "Input.default"}),
+              ("gate", FullyConnected(12, "linear", fused=fused), {"default": "embed.default"}),
+              ("first", GatedResidual("sigmoid", 0.5), {"block": "embed.default", "gate": "gate.default", "x": "embed.default"}),
+              ("second", GatedResidual("tanh"), {"block": "first.default", "gate": "first.default", "x": "first.default"}),
+              ("third", GatedResidual("swish"), {"block": "second.default", "gate": "second.default", "x": "second.residual"}),
+              ("out", FullyConnected(5, "linear", fused=fused), {"default": "third.default"}),
+              ("ce", SoftmaxCE(fused=fused), {"default": "out.default", "targets": "Input.targets"}),
+              ("loss", Loss(), {"default": "ce.loss"})]
+    net = Net(handler, layers)
+    rng = np.random.RandomState(4)
+    data = {"default": rng.standard_normal((3, 4, 9)).astype(F32), "targets": rng.randint(0, 5, (3, 4, 1)).astype(F32)}
+    net.provide_external_data(data)
+    return net, data, 0.5 * rng.standard_normal(net.parameter_count()) + 0.2
+
+
+def test_inputs_from_one_output():
+    net, data, params = shared_sources(SequenceRefHandler(np.float64, seed=1), False)
+    loss_of(net, data, params)
+    net.backward_pass()
+    grads = net.handler.get_numpy_copy(net.gradients)
+    for name, (a, b, _) in net.parameter_slices().items():
+        for i in np.unique(np.linspace(a, b - 1, min(b - a, 5)).astype(int)):
+            moved = []
+            for sign in (1, -1):
+                p = params.copy()
+                p[i] += sign * 1e-6
+                moved.append(loss_of(net, data, p))
+            np.testing.assert_allclose(grads[i], (moved[0] - moved[1]) / 2e-6, rtol=1e-4, atol=1e-7, err_msg=name)
+
+
+@pytest.mark.gpu
+def test_inputs_from_one_output_on_the_gpu(hip):
+    # 2e-4 of each array's scale, as for the network below
+    got = []
+    for handler, fused in ((hip, True), (SequenceRefHandler(np.float64, seed=1), False)):
+        net, _, params = shared_sources(handler, fused)
+        net.set_parameters(params if handler is not hip else params.astype(F32))
+        net.forward_pass(training_pass=True)
+        net.backward_pass()
+        got.append((net.handler.get_numpy_copy(net.gradients), net.parameter_slices()))
+    for name, (a, b, _) in got[1][1].items():
+        want = got[1][0][a:b]
+        assert np.abs(got[0][0][a:b] - want).max() <= 2e-4 * np.abs(want).max(), name
 
 
 def test_orthogonal_stepper_groups_equal_neighbours():

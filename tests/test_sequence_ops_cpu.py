@@ -111,6 +111,11 @@ def refused(h):
         ("three axes", lambda: gate("linear", stack, None, stack, w, w, stack, stack)),
         ("no dgate", lambda: gate_back("linear", m, m, w, w, m, m, m, m, None, m, w, w)),
         ("no dh", lambda: gate_back("linear", m, m, w, w, m, m, None, m, m, m, w, w)),
+        ("y is h", lambda: gate("linear", m, m, m, w, w, m, m)),
+        ("dblock is dgate", lambda: gate_back("linear", m, m, w, w, m, m, m, m, m, A(4, 6), A(6), A(6))),
+        ("dgate overlaps dx",
+         lambda: gate_back("linear", m, m, w, w, m, m, m, m, flat[0:24].reshape((4, 6)), flat[6:30].reshape((4, 6)), A(6), A(6))),
+        ("dpost is dpre", lambda: gate_back("linear", m, m, w, w, m, m, m, m, A(4, 6), A(4, 6), w, w)),
         ("norm weight", lambda: h.rms_norm_forward(m, A(7), m)),
         ("norm out", lambda: h.rms_norm_forward(m, w, n)),
         ("norm gradient", lambda: h.rms_norm_backward(m, w, n, m, w)),
