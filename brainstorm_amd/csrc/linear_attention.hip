@@ -32,8 +32,8 @@
 //   one step, 4096 sequences of 128 x 128: the state in and out, 537 MB: 106 us, 5.1 TB/s; 8 sequences: a launch, 3.7 us
 //   16 sequences of 8192 steps of 64: 70 us in three launches (states of the segments 22, scan 6, pass 45); 134 MB would
 //     take 26 us, but a segment's chunks wait for each other
-//   128 sequences of 1024 steps of 128: forward 153 us, backward 464; 30 GFLOP that cannot be left out take 198 us; 60 % of
-//     the matrix rate inside a pass, the rest is the derivative by the decay, a quarter of the work
+//   128 sequences of 1024 steps of 128: forward 153 us, backward 464; 30 GFLOP that cannot be left out take 198 us; matrix
+//     cores 44 % (one wavefront a SIMD) to 55 % (two) busy, a quarter of the work is the derivative by the decay
 //   800 sequences of 100 steps of 125, all scores: forward 66 us, backward 168 us
 #include "common.h"
 
@@ -130,7 +130,8 @@ struct Passes {
     PassArgs pass[2];
 };
 
-// NI: tiles of 16 features of q and k held (di <= 16 NI). NW: wavefronts, each with 16 features of v (dj <= 16 NW). TAN:
+// NI: tiles of 16 features of q and k held (di <= 16 NI). NW: wavefronts, each with 16 features of v, blockIdx.z: from which
+// 16 NW of them on (dj <= 16 NW gridDim.z). TAN:
 // with the derivative by the decay. STATE: only the state behind a segment that starts from zero.
 //
 // q and k of a chunk are staged in LDS (every wavefront reads all of both, as operands of the scores, of q C and of

@@ -20,8 +20,8 @@ def pytest_configure(config):
 
 @pytest.fixture(scope="module", autouse=True)
 def earlier_garbage():
-    """Collects what the tests of other files left in cycles. A collection in the middle of a test frees their arrays, and
-    a free between two calls ends a sequence of the fusing window, whose launches some tests count."""
+    """Collects what the tests of other files left in cycles, handlers above all. Collected in the middle of a test they
+    release their generators, which enqueues what the fusing window holds, and some tests count its launches."""
     gc.collect()
 
 
