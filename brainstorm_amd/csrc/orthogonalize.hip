@@ -196,7 +196,13 @@ enum { kGram, kPoly, kNext, kLast };
 // the result, rows 4 (l / 16) + r, column l % 16. WM x WN wavefronts share the tile; G such groups share the summed axis
 // (every G-th step of 32 each) and add their sums up in LDS at the end: a small tile's step is a chain of waits, which
 // other groups' steps fill. Loads go straight to LDS, a block of a plane per instruction, STAGES - 1 steps ahead.
-template <int T, int WM, int WN, int G, int STAGES, int MODE>
+//
+// FINE: lo lo is taken too, and all that is not hi hi is summed apart, where sums are 2^11 times smaller and so is what they
+// round off. Sums over few entries need it: what three products leave out and round does not average out there. (Error against
+// 64 bits over that of the same steps in plain float32, 150 matrices of random sides from 8 to 1200: smaller sides up to 64,
+// median 1.04, largest 1.84; with it 0.83 and 1.25; longer ones 0.47 without. 2 x 53 x 16: 64 us, with it 67; 4 x 1000 x 1000
+// would take 6 % more.)
+template <int T, int WM, int WN, int G, int STAGES, int MODE, bool FINE>
 __global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_product_kernel(ProductArgs a) {
     constexpr int kWaves = WM * WN;                      // of one group
     constexpr int X = T / WM / 16, Y = T / WN / 16;      // tiles of 16 on the sides of a wavefront's part
@@ -260,6 +266,12 @@ __global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_produ
     for (int x = 0; x < X; ++x)
 #pragma unroll
         for (int y = 0; y < Y; ++y) acc[x][y] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    f4 fine[FINE ? X : 1][FINE ? Y : 1];
+    if constexpr (FINE)
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int y = 0; y < Y; ++y) fine[x][y] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
     // steps of this group; all groups go through as many as the first, the last one perhaps without products
     const int blocks_k = a.k / 32, steps = (blocks_k + G - 1) / G;
@@ -304,10 +316,19 @@ __global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_produ
             __builtin_amdgcn_sched_barrier(0);         // the reads above are under way during the products below
             if (G > 1 && s >= own) continue;
             const Row& p = row[x & 1];
+            if constexpr (FINE) {
 #pragma unroll
-            for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.lo, now.hi[y], acc[x][y]);
+                for (int y = 0; y < Y; ++y) fine[x][y] = mfma(p.lo, now.lo[y], fine[x][y]);
 #pragma unroll
-            for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.hi, now.lo[y], acc[x][y]);
+                for (int y = 0; y < Y; ++y) fine[x][y] = mfma(p.lo, now.hi[y], fine[x][y]);
+#pragma unroll
+                for (int y = 0; y < Y; ++y) fine[x][y] = mfma(p.hi, now.lo[y], fine[x][y]);
+            } else {
+#pragma unroll
+                for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.lo, now.hi[y], acc[x][y]);
+#pragma unroll
+                for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.hi, now.lo[y], acc[x][y]);
+            }
 #pragma unroll
             for (int y = 0; y < Y; ++y) acc[x][y] = mfma(p.hi, now.hi[y], acc[x][y]);
             __builtin_amdgcn_sched_barrier(0);
@@ -325,6 +346,11 @@ __global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_produ
         step(s, even, odd);
         if (s + 1 < steps) step(s + 1, odd, even);
     }
+    if constexpr (FINE)
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int y = 0; y < Y; ++y) acc[x][y] += fine[x][y];
 
     // a 16 x 16 tile of the result: rows i .. i + 3, column j
     auto finish = [&](f4 v, int i, int j) {
@@ -405,11 +431,13 @@ __global__ __launch_bounds__(WM * WN * G * kWave, WM * WN * G / 4) void ns_produ
     }
 }
 
-template <int T, int WM, int WN, int G, int STAGES, int MODE>
+template <int T, int WM, int WN, int G, int STAGES, int MODE, bool FINE = false>
 void launch_tiles(const ProductArgs& a, unsigned count) {
-    hipLaunchKernelGGL((ns_product_kernel<T, WM, WN, G, STAGES, MODE>), dim3(a.tiles * count), dim3(WM * WN * G * kWave), 0,
+    hipLaunchKernelGGL((ns_product_kernel<T, WM, WN, G, STAGES, MODE, FINE>), dim3(a.tiles * count), dim3(WM * WN * G * kWave), 0,
                        ctx().stream, a);
 }
+
+constexpr int kFineMost = 128;      // matrices with smaller sides up to it take the finer sums, in tiles of 64
 
 // The tile side: what 32 entries of the summed axis cost with one tile on every compute unit, in hundredths of a
 // microsecond, times the rounds that the tiles take. Measured (4096 x 4096: 256 against 192 and 128 for the full product
@@ -418,6 +446,7 @@ void launch_tiles(const ProductArgs& a, unsigned count) {
 // whole; where there is at most one for each, four groups share its summed axis (784 x 1200: 13 us, one group 20).
 template <int MODE>
 int launch_product(ProductArgs a, unsigned count) {
+    const bool fine = a.used_p <= kFineMost;            // the smaller side
     const int64_t cus = ctx().num_cus;
     constexpr int kTiles[] = {256, 192, 128, 64}, kCost[] = {260, 160, 83, 30};
     int best = 0;                       // (a launch has fewer than 2^32 threads: up to 512 of them for a tile)
@@ -427,7 +456,7 @@ int launch_product(ProductArgs a, unsigned count) {
         const int64_t tiles = MODE == kGram || MODE == kPoly ? side * (side + 1) / 2 : side * other;
         const int64_t all = tiles * count;
         const double rounds = kTiles[n] == 64 ? static_cast<double>(all > cus ? all : cus) / cus : static_cast<double>(ceil_div(all, cus));
-        if (all > 0x7fffff || (best && rounds * kCost[n] >= least)) continue;
+        if (all > 0x7fffff || (fine && kTiles[n] != 64) || (best && rounds * kCost[n] >= least)) continue;
         least = rounds * kCost[n];
         best = kTiles[n];
         a.tiles_p = static_cast<int>(side);
@@ -438,7 +467,10 @@ int launch_product(ProductArgs a, unsigned count) {
         case 192: launch_tiles<192, 2, 4, 1, 3, MODE>(a, count); break;
         case 128: launch_tiles<128, 2, 2, 2, 2, MODE>(a, count); break;
         case 64:
-            if (static_cast<int64_t>(a.tiles) * count > cus) launch_tiles<64, 2, 2, 1, 2, MODE>(a, count);
+            if (fine) {
+                if (static_cast<int64_t>(a.tiles) * count > cus) launch_tiles<64, 2, 2, 1, 2, MODE, true>(a, count);
+                else launch_tiles<64, 2, 2, 4, 2, MODE, true>(a, count);
+            } else if (static_cast<int64_t>(a.tiles) * count > cus) launch_tiles<64, 2, 2, 1, 2, MODE>(a, count);
             else launch_tiles<64, 2, 2, 4, 2, MODE>(a, count);
             break;
         default: return set_error(BSHIP_ERR_BAD_DIMENSION, "orthogonalize: the matrices exceed one launch");
