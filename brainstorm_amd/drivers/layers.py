@@ -44,6 +44,13 @@ def flatten_all_but_last(a):
     return a.reshape((_prod(a.shape[:-1]), a.shape[-1]))
 
 
+def same_memory(a, b):
+    """Whether two views begin at the same element (the sinks of a source with context slots get a view each)."""
+    def address(v):
+        return v._address() if hasattr(v, "_address") else v.__array_interface__["data"][0]
+    return a is b or (a.size > 0 and b.size > 0 and address(a) == address(b))
+
+
 class Buf:
     """Description of one buffer of a layer: per-sample feature shape, whether it scales with
     time and batch ('TB'), extra context time steps, and whether only the backward pass uses it."""
@@ -729,7 +736,7 @@ class GatedResidual(Layer):
         block, gate = (flatten_time_and_features(buffers.inputs[n]) for n in ("block", "gate"))
         sources = [buffers.input_deltas[n] for n in ("block", "gate", "x")]
         deltas = [flatten_time_and_features(d) for d in sources]
-        shared = [n for n in (1, 2) if any(sources[n] is d for d in sources[:n])]     # two inputs from one output
+        shared = [n for n in (1, 2) if any(same_memory(sources[n], d) for d in sources[:n])]     # two inputs from one output
         for n in shared:
             deltas[n] = _h.zeros(deltas[n].shape)
         dblock, dgate, dx = deltas

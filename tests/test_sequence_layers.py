@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from brainstorm_amd.drivers import configs
-from brainstorm_amd.drivers.layers import FullyConnected, GatedResidual, Input, Loss, SoftmaxCE
+from brainstorm_amd.drivers.layers import FullyConnected, GatedResidual, Input, Loss, Lstm, SoftmaxCE
 from brainstorm_amd.drivers.net import MomentumStepper, Net, OrthogonalStepper
 from oracle.sequence_ops import SequenceRefHandler
 
@@ -219,3 +219,63 @@ def test_orthogonal_stepper_trains_any_network(hip):
 def test_momentum_stepper_is_unchanged():
     stepper = MomentumStepper(0.1, 0.5)
     assert (stepper.learning_rate, stepper.momentum, stepper.scale_learning_rate, stepper.fused) == (0.1, 0.5, True, False)
+
+
+class OutputsApart(SequenceRefHandler):
+    """The oracle with HipHandler's refusal of outputs that share memory."""
+
+    def gated_residual_backward(self, activation, block, gate, post_weight, pre_weight, y, dy, dh, dblock, dgate, dx, *args,
+                                **kwargs):
+        outputs = [a for a in (dblock, dgate, dx) if a is not None]
+        if any(np.shares_memory(a, b) for n, a in enumerate(outputs) for b in outputs[:n]):
+            raise ValueError("two outputs overlap")
+        super().gated_residual_backward(activation, block, gate, post_weight, pre_weight, y, dy, dh, dblock, dgate, dx, *args,
+                                        **kwargs)
+
+
+def recurrent_source(handler, fused, inputs):
+    """An Lstm, whose buffers have a context slot, as the source of a GatedResidual's `inputs`."""
+    layers = [("Input", Input({"default": (9,), "targets": (1,)}), {}),
+              ("lstm", Lstm(12, fused=fused), {"default": "Input.default"}),
+              ("other", FullyConnected(12, "linear", fused=fused), {"default": "lstm.default"}),
+              ("end", GatedResidual("swish"), {n: ("lstm" if n in inputs else "other") + ".default"
+                                               for n in ("block", "gate", "x")}),
+              ("out", FullyConnected(5, "linear", fused=fused), {"default": "end.default"}),
+              ("ce", SoftmaxCE(fused=fused), {"default": "out.default", "targets": "Input.targets"}),
+              ("loss", Loss(), {"default": "ce.loss"})]
+    net = Net(handler, layers)
+    rng = np.random.RandomState(7)
+    data = {"default": rng.standard_normal((3, 4, 9)).astype(F32), "targets": rng.randint(0, 5, (3, 4, 1)).astype(F32)}
+    net.provide_external_data(data)
+    return net, data, 0.5 * rng.standard_normal(net.parameter_count()) + 0.2
+
+
+SHARED = [("block", "gate", "x"), ("block", "gate"), ("block", "x"), ("gate", "x")]
+
+
+@pytest.mark.parametrize("inputs", SHARED)
+def test_inputs_from_one_recurrent_output(inputs):
+    net, data, params = recurrent_source(OutputsApart(np.float64, seed=1), False, inputs)
+    loss_of(net, data, params)
+    net.backward_pass()
+    want, want_data, _ = recurrent_source(SequenceRefHandler(np.float64, seed=1), False, inputs)
+    loss_of(want, want_data, params)
+    want.backward_pass()
+    np.testing.assert_allclose(net.handler.get_numpy_copy(net.gradients), want.handler.get_numpy_copy(want.gradients),
+                               rtol=1e-12, atol=1e-14)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inputs", SHARED)
+def test_inputs_from_one_recurrent_output_on_the_gpu(hip, inputs):
+    # 2e-4 of each array's scale, as for the networks above
+    got = []
+    for handler, fused in ((hip, True), (SequenceRefHandler(np.float64, seed=1), False)):
+        net, _, params = recurrent_source(handler, fused, inputs)
+        net.set_parameters(params if handler is not hip else params.astype(F32))
+        net.forward_pass(training_pass=True)
+        net.backward_pass()
+        got.append((net.handler.get_numpy_copy(net.gradients), net.parameter_slices()))
+    for name, (a, b, _) in got[1][1].items():
+        want = got[1][0][a:b]
+        assert np.abs(got[0][0][a:b] - want).max() <= 2e-4 * np.abs(want).max(), name
