@@ -1408,15 +1408,22 @@ class HipHandler(Handler):
         return time, batch, heads, dk, dv
 
     @staticmethod
-    def _no_overlap(op, outputs, inputs, allowed=()):
-        """Refuses outputs that share memory with another operand, but for the pairs (output, input) `allowed`."""
+    def _no_overlap(op, outputs, inputs, allowed=(), in_place=()):
+        """Refuses outputs that share memory with another operand, but for the pairs (output, input) `allowed` and, for
+        each pair (outputs, inputs) of lists in `in_place`, those of the outputs that are one of the inputs."""
+        if _fastcall.apart(*outputs, *inputs):
+            return
         for n, a in enumerate(outputs):
             if a is None or not a.size:
                 continue
             first, end = a.ptr, a.ptr + 4 * a.size
             for b in inputs:
-                if b is not None and b.ptr < end and first < b.ptr + 4 * b.size and (a, b) not in allowed:
-                    raise ValueError("%s: an output overlaps another operand" % op)
+                if b is None or b.ptr >= end or first >= b.ptr + 4 * b.size or (a, b) in allowed:
+                    continue
+                if a.ptr == b.ptr and a.size == b.size and any(
+                        any(a is x for x in these) and any(b is x for x in those) for these, those in in_place):
+                    continue
+                raise ValueError("%s: an output overlaps another operand" % op)
             for b in outputs[n + 1:]:
                 if b is not None and b.ptr < end and first < b.ptr + 4 * b.size:
                     raise ValueError("%s: two outputs overlap" % op)
@@ -1472,11 +1479,14 @@ class HipHandler(Handler):
         norms behind a block and before the next one with the block's gate, in one pass. Matrices are
         (rows, width), weights have width elements, rms(v) = sqrt(mean(v * v) + epsilon) over a row. gate may
         be None (no gate), pre_weight and h together (no norm behind). Activations: those of act_func and
-        'swish'. An output may be an input, but y and h are two arrays."""
+        'swish'. An output may be block, gate or x; y and h are two arrays, and any other overlap is refused."""
         code = self._gate_code("gated_residual_forward", activation)
         self._gate_shapes("gated_residual_forward", (block, x, y), (gate,), (post_weight,), pre_weight, (h,))
-        if pre_weight is not None:
-            self._no_overlap("gated_residual_forward", [y, h], ())
+        if pre_weight is None:
+            h = None
+        if not _fastcall.apart(block, gate, x, post_weight, pre_weight, y, h):
+            self._no_overlap("gated_residual_forward", [y, h], [block, gate, x, post_weight, pre_weight],
+                             in_place=[([y, h], [block, gate, x])])
         rows, width = x.shape
         self._call(self._lib.bship_gated_residual_fwd_f32(
             code, block.ptr, self._ptr(gate), x.ptr, post_weight.ptr, self._ptr(pre_weight),
@@ -1487,14 +1497,19 @@ class HipHandler(Handler):
         """The gradients of gated_residual_forward. dblock, dgate and dx are added to what they hold (as a layer
         adds to its input deltas) or, with accumulate=False, overwritten; the weights' gradients are
         overwritten. gate and dgate are None together, and so are pre_weight, dh and dpre_weight. No output may be
-        another one: a block's source that is also the gate's needs an array for each."""
+        another one: a block's source that is also the gate's needs an array for each. dblock, dgate and dx may be
+        block, gate, y, dy or dh, and a weight's gradient a weight; any other overlap is refused."""
         op = "gated_residual_backward"
         code = self._gate_code(op, activation)
         self._gate_shapes(op, (block, dy, dblock, dx), (gate, dgate), (post_weight, dpost_weight), pre_weight,
                           (y, dh), (dpre_weight,))
         if (gate is None) != (dgate is None):
             raise ValueError("%s: gate and dgate go together" % op)
-        self._no_overlap(op, [dblock, dgate, dx, dpost_weight, dpre_weight if pre_weight is not None else None], ())
+        matrices, weights = [block, gate, y if pre_weight is not None else None, dy,
+                             dh if pre_weight is not None else None], [post_weight, pre_weight]
+        outputs, gradients = [dblock, dgate, dx], [dpost_weight, dpre_weight if pre_weight is not None else None]
+        self._no_overlap(op, outputs + gradients, matrices + weights,
+                         in_place=[(outputs, matrices), (gradients, weights)])
         rows, width = dx.shape
         self._call(self._lib.bship_gated_residual_bwd_f32(
             code, block.ptr, self._ptr(gate), post_weight.ptr, self._ptr(pre_weight),
@@ -1509,29 +1524,37 @@ class HipHandler(Handler):
         shape = matrices[0].shape
         if len(shape) != 2:
             raise ValueError("%s: matrices are wanted, got %r" % (op, tuple(shape)))
-        given = [m for m in optional if m is not None]
-        vectors = list(weights)
         if pre_weight is not None:
-            if any(m is None for m in tuple(pre_matrices) + tuple(pre_weights)):
+            if None in pre_matrices or None in pre_weights:
                 raise ValueError("%s: an operand of the norm before the next block is missing" % op)
-            given += pre_matrices
-            vectors += [pre_weight] + list(pre_weights)
-        if any(m.shape != shape for m in list(matrices) + given) or any(w.size != shape[1] for w in vectors):
-            raise _mismatch(op, *(list(matrices) + given + vectors))
+            matrices += pre_matrices
+            weights += (pre_weight,) + pre_weights
+        for m in matrices + optional:
+            if m is not None and m.shape != shape:
+                break
+        else:
+            for w in weights:
+                if w.size != shape[1]:
+                    break
+            else:
+                return
+        raise _mismatch(op, *[a for a in matrices + optional + weights if a is not None])
 
     def rms_norm_forward(self, x, weight, out, epsilon=1e-6):
         """out = weight * x / sqrt(mean(x * x) + epsilon) over the rows of a (rows, width) matrix: the norm before the
-        first block."""
+        first block. out may be x."""
         self._gate_shapes("rms_norm_forward", (x, out), (), (weight,), None, ())
+        self._no_overlap("rms_norm_forward", [out], [x, weight], in_place=[([out], [x])])
         rows, width = x.shape
         self._call(self._lib.bship_gated_residual_fwd_f32(3, None, None, x.ptr, None, weight.ptr, None, out.ptr, rows,
                                                           width, 1.0, epsilon))
 
     def rms_norm_backward(self, x, weight, dout, dx, dweight, epsilon=1e-6, accumulate=True):
         """The gradients of rms_norm_forward; dx is added to what it holds or, with accumulate=False, overwritten,
-        dweight is overwritten."""
+        dweight is overwritten. dx may be x or dout, dweight may be weight."""
         self._gate_shapes("rms_norm_backward", (x, dout, dx), (), (weight, dweight), None, ())
-        self._no_overlap("rms_norm_backward", [dx, dweight], ())
+        self._no_overlap("rms_norm_backward", [dx, dweight], [x, dout, weight],
+                         in_place=[([dx], [x, dout]), ([dweight], [weight])])
         rows, width = x.shape
         self._call(self._lib.bship_gated_residual_bwd_f32(3, None, None, None, weight.ptr, x.ptr, None, dout.ptr, None,
                                                           None, dx.ptr, None, dweight.ptr, rows, width, 1.0, epsilon,

@@ -732,17 +732,17 @@ int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* 
  *     rms(v) = sqrt(mean(v * v) + epsilon) over a row
  * act is a BSHIP_ACT_* code, BSHIP_ACT_SWISH included. gate NULL: no gate. pre NULL: no norm behind, h
  * is not written. block NULL: only the norm, h = pre * x / rms(x), y is not written. An output may be
- * one of the inputs, but not the other output. Recordable. */
+ * block, gate or x, but neither the other output nor anything else that overlaps an operand. Recordable. */
 int bship_gated_residual_fwd_f32(int act, const float* block, const float* gate, const float* x,
                                  const float* post, const float* pre, float* y, float* h,
                                  int64_t rows, int64_t width, float residual_scale,
                                  float epsilon);
 /* Its gradients, from dy and dh (those of y and h; dy may be NULL if pre is given, dh is not read if
  * pre is NULL). dblock, dgate, dx are added to what they hold if accumulate is not 0 (as a layer's
- * backward pass adds to its input deltas), else overwritten, and may then be one of the inputs;
+ * backward pass adds to its input deltas), else overwritten, and may be block, gate, y, dy or dh;
  * dpost and dpre (width) are overwritten, summed over the rows in a fixed order. y is the forward
- * pass's y (its x if block is NULL); it is not read if pre is NULL. No output may be another one. Takes
- * scratch from the pool; recordable. */
+ * pass's y (its x if block is NULL); it is not read if pre is NULL. No output may be another one or
+ * overlap an operand otherwise. Takes scratch from the pool; recordable. */
 int bship_gated_residual_bwd_f32(int act, const float* block, const float* gate,
                                  const float* post, const float* pre, const float* y,
                                  const float* dy, const float* dh, float* dblock, float* dgate,

@@ -145,3 +145,99 @@ def test_unknown_gate_activation(trace):
     m, w = h.allocate((4, 6)), h.allocate((6,))
     with pytest.raises(ValueError):
         h.gated_residual_forward("softplus", m, m, m, w, w, m, m)
+
+
+def overlapping(h):
+    """Calls of the norms whose outputs share memory with an input that they are not."""
+    A = lambda *shape: h.allocate(shape)
+    flat = A(200)
+    at = lambda first: flat[first:first + 24].reshape((4, 6))
+    weight = lambda first: flat[first:first + 6]
+    m, w = A(4, 6), A(6)
+    gate, back = h.gated_residual_forward, h.gated_residual_backward
+    fresh = lambda: (A(4, 6), A(4, 6), A(4, 6), A(6), A(6))
+
+    def gradients(where, first):
+        grads = list(fresh())
+        grads[where] = at(first) if where < 3 else weight(first)
+        return grads
+
+    calls = []
+    for shift in (1, 6):                        # by an element, by a row; up and down
+        for a, b in ((0, shift), (shift, 0)):
+            calls += [
+                ("y over x", lambda a=a, b=b: gate("tanh", m, m, at(a), w, w, at(b), A(4, 6))),
+                ("y over block", lambda a=a, b=b: gate("tanh", at(a), m, m, w, w, at(b), A(4, 6))),
+                ("y over gate, no norm behind", lambda a=a, b=b: gate("tanh", m, at(a), m, w, None, at(b), None)),
+                ("h over x", lambda a=a, b=b: gate("tanh", m, m, at(a), w, w, A(4, 6), at(b))),
+                ("the norm's out over x", lambda a=a, b=b: h.rms_norm_forward(at(a), w, at(b))),
+                ("the norm's dx over x", lambda a=a, b=b: h.rms_norm_backward(at(a), w, m, at(b), A(6))),
+                ("the norm's dx over dout", lambda a=a, b=b: h.rms_norm_backward(m, w, at(a), at(b), A(6)))]
+            for where, name in enumerate(("dblock", "dgate", "dx")):
+                for n, of in enumerate(("block", "gate", "y", "dy", "dh")):
+                    def call(where=where, n=n, a=a, b=b):
+                        x = [m] * 5
+                        x[n] = at(a)
+                        back("tanh", x[0], x[1], w, w, x[2], x[3], x[4], *gradients(where, b))
+                    calls.append(("%s over %s" % (name, of), call))
+    calls += [
+        ("y over post", lambda: gate("tanh", m, m, m, weight(6), w, at(0), A(4, 6))),
+        ("h over pre", lambda: gate("tanh", m, m, m, w, weight(6), A(4, 6), at(0))),
+        ("y is post", lambda: gate("tanh", m[:1], m[:1], m[:1], w, A(6), w.reshape((1, 6)), A(1, 6))),
+        ("dx over pre", lambda: back("tanh", m, m, w, weight(6), m, m, m, *gradients(2, 0))),
+        ("dblock over post", lambda: back("tanh", m, m, weight(6), w, m, m, m, *gradients(0, 0))),
+        ("dpost over dy", lambda: back("tanh", m, m, w, w, m, at(0), m, *gradients(3, 6))),
+        ("dpre over post", lambda: back("tanh", m, m, weight(1), w, m, m, m, *gradients(4, 0))),
+        ("the norm's out over weight", lambda: h.rms_norm_forward(m, weight(6), at(0))),
+        ("the norm's dx over weight", lambda: h.rms_norm_backward(m, weight(6), m, at(0), A(6))),
+        ("the norm's dweight over x", lambda: h.rms_norm_backward(at(0), w, m, A(4, 6), weight(6))),
+    ]
+    return calls
+
+
+def test_outputs_that_overlap_an_input_are_refused(trace):
+    from brainstorm_amd import HipHandler
+    h = HipHandler(seed=1)
+    for what, call in overlapping(h):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+            pytest.fail("not refused: " + what)
+
+
+def test_outputs_in_an_inputs_place_reach_the_library(trace):
+    # the calls that stay allowed: the stand-in library has none of these entry points, which is how a call that gets there ends
+    from brainstorm_amd import HipHandler
+    h = HipHandler(seed=1)
+    A = lambda *shape: h.allocate(shape)
+    for inputs in range(5):
+        for output in range(3):
+            x, grads = [A(4, 6) for _ in range(5)], [A(4, 6) for _ in range(3)]
+            grads[output] = x[inputs]
+            w = [A(6), A(6)]
+            for accumulate in (False, True):
+                with pytest.raises(AttributeError, match="bship_gated_residual_bwd_f32"):
+                    h.gated_residual_backward("tanh", x[0], x[1], *w, *x[2:], *grads, *w, accumulate=accumulate)
+    for inputs in range(3):
+        x = [A(4, 6) for _ in range(3)]
+        for outputs in ((x[inputs], A(4, 6)), (A(4, 6), x[inputs]), (x[inputs], x[inputs - 1])):
+            with pytest.raises(AttributeError, match="bship_gated_residual_fwd_f32"):
+                h.gated_residual_forward("tanh", *x, A(6), A(6), *outputs)
+    m, w = A(4, 6), A(6)
+    with pytest.raises(AttributeError, match="bship_gated_residual_fwd_f32"):
+        h.rms_norm_forward(m, w, m)
+    for x, dout in ((m, A(4, 6)), (A(4, 6), m)):
+        with pytest.raises(AttributeError, match="bship_gated_residual_bwd_f32"):
+            h.rms_norm_backward(x, w, dout, m, w)
+
+
+def test_apart():
+    from brainstorm_amd._fastcall import apart
+    from brainstorm_amd.device_array import DeviceArray
+    a = lambda ptr, n: DeviceArray(ptr, (n,), None)
+    assert apart() and apart(None) and apart(a(1024, 4), None, a(1040, 4), a(1008, 4), a(1028, 0), a(0, 0), a(0, 0))
+    for ptr, n in ((1024, 4), (1020, 2), (1036, 1), (1000, 100), (1028, 1)):
+        assert not apart(a(1024, 4), a(ptr, n)) and not apart(a(ptr, n), a(5000, 3), None, a(1024, 4))
+    with pytest.raises(TypeError, match="at most 24"):
+        apart(*[None] * 25)
+    with pytest.raises(AttributeError):
+        apart(a(1024, 4), 7)
