@@ -25,7 +25,7 @@ from ._lib import (ABS, ADD, ADD_IF, ADD_ST, COPY_IF, DIV, EL, EL_DERIV, FILL_IF
                    MULT_ADD_ST, MULT_ST, PITCHED_BINARY, PITCHED_CLIP, PITCHED_COND, PITCHED_DERIV,
                    PITCHED_FILL, PITCHED_MULT_ADD, PITCHED_SCALAR, PITCHED_UNARY, REL, REL_DERIV, SIGMOID,
                    SIGMOID_DERIV, SIGN, SQRT, SUB, TANH, TANH_DERIV)
-from .device_array import DeviceArray, PitchedDeviceArray, _Block, _prod
+from .device_array import ITEMSIZE, DeviceArray, PitchedDeviceArray, _Block, _prod
 from .handler_api import Handler
 
 SEED_RANGE = (0, 1000000000)   # brainstorm/randomness.py:16
@@ -193,6 +193,24 @@ def _native_pitched_table():
     return table
 
 
+def _share_elements(a, b):
+    """Whether two arrays, each dense or row-pitched, have an element in common (sure to be found; views of different
+    pitches count as overlapping wherever their spans meet)."""
+    if not a.size or not b.size:
+        return False
+    (rows_a, run_a, pitch_a), (rows_b, run_b, pitch_b) = [
+        (v.rows, v.run, v.pitch) if type(v) is PitchedDeviceArray and v.rows > 1 else (1, v.size, None) for v in (a, b)]
+    pitch = pitch_a or pitch_b or 1
+    off = (b._address() - a._address()) // ITEMSIZE              # of b's first element behind a's
+    if rows_a > 1 and rows_b > 1 and pitch_a != pitch_b:
+        return -((rows_b - 1) * pitch_b + run_b) < off < (rows_a - 1) * pitch_a + run_a
+    # a's row i and b's row i + k meet if -run_b < off + k pitch < run_a
+    least, most = (-run_b - off) // pitch + 1, -((off - run_a) // pitch) - 1
+    if rows_a == 1 and rows_b == 1:
+        return -run_b < off < run_a
+    return max(least, 1 - rows_a) <= min(most, rows_b - 1)
+
+
 class HipHandler(Handler):
     __undescribed__ = {'context', 'dtype', 'EMPTY', 'rnd'}
 
@@ -279,6 +297,10 @@ class HipHandler(Handler):
         "rms_norm_backward": ("dx", "dweight"),
         "orthogonalize": ("out",), "orthogonal_update": ("velocity", "parameters"),
     }
+    # operations that refuse outputs which overlap each other: behind dense temporaries they could not see it
+    _OUTPUTS_APART = frozenset(("linear_attention_forward", "linear_attention_step", "linear_attention_backward",
+                                "gated_residual_forward", "gated_residual_backward", "rms_norm_backward",
+                                "orthogonal_update"))
 
     def _install_pitched_wrappers(self):
         import functools
@@ -537,6 +559,11 @@ class HipHandler(Handler):
                 return native(self, bound.arguments)
             except _NoNativePath:
                 pass                                 # e.g. operands of different row lengths
+        if fn.__name__ in self._OUTPUTS_APART:
+            outputs = [bound.arguments[k] for k in written if bound.arguments.get(k) is not None]
+            for n, a in enumerate(outputs):
+                if any(_share_elements(a, b) for b in outputs[:n]):
+                    raise ValueError("%s: two outputs overlap" % fn.__name__)
         pitched = [(k, a) for k, a in bound.arguments.items() if type(a) is PitchedDeviceArray]
         temps = {}
         for name, a in pitched:

@@ -241,3 +241,40 @@ def test_apart():
         apart(*[None] * 25)
     with pytest.raises(AttributeError):
         apart(a(1024, 4), 7)
+
+
+def test_shared_elements_of_row_pitched_views():
+    # every pair of a few dense and pitched views of one buffer, against the sets of their elements
+    from brainstorm_amd.device_array import DeviceArray, PitchedDeviceArray
+    from brainstorm_amd.hip_handler import _share_elements
+    views = []
+    for first in (0, 1, 3, 5, 7, 12, 20, 29):
+        for n in (0, 1, 2, 6, 11):
+            views.append((DeviceArray(4096 + 4 * first, (n,), None), set(range(first, first + n))))
+        for rows, run, pitch in ((1, 3, 7), (2, 3, 7), (4, 1, 7), (3, 6, 7), (3, 2, 5), (2, 4, 5)):
+            elements = {first + r * pitch + c for r in range(rows) for c in range(run)}
+            views.append((PitchedDeviceArray(4096 + 4 * first, (rows, run), pitch, None, None), elements))
+    for a, of_a in views:
+        for b, of_b in views:
+            pitches = {v.pitch for v in (a, b) if type(v) is PitchedDeviceArray and v.rows > 1}
+            if len(pitches) < 2:
+                assert _share_elements(a, b) == bool(of_a & of_b), (a, b)
+            else:                                         # may be taken for overlapping, never for apart
+                assert _share_elements(a, b) or not of_a & of_b, (a, b)
+
+
+def test_row_pitched_outputs_that_overlap_are_refused(trace):
+    from brainstorm_amd import HipHandler
+    h = HipHandler(seed=1, pitched_views=True)
+    A = lambda *shape: h.allocate(shape)
+    hub, m, w = A(4, 20), A(4, 6), A(6)
+    x, s = A(5, 2, 8), A(2, 2, 4, 4)
+    wide = A(5, 2, 20)
+    with pytest.raises(ValueError, match="two outputs overlap"):
+        h.gated_residual_forward("tanh", m, m, m, w, w, hub[:, 2:8], hub[:, 7:13])
+    with pytest.raises(ValueError, match="two outputs overlap"):
+        h.gated_residual_backward("tanh", m, m, w, w, m, m, m, hub[:, 2:8], A(4, 6), hub[:, 3:9], A(6), A(6))
+    with pytest.raises(ValueError, match="two outputs overlap"):
+        h.linear_attention_backward(x, x, x, A(2), x, wide[:, :, :8], wide[:, :, 8:16], wide[:, :, 12:20])
+    with pytest.raises(ValueError, match="two outputs overlap"):
+        h.orthogonal_update(0.9, -0.1, m, hub[:, 1:7], hub[:, :6])
