@@ -753,13 +753,19 @@ class GatedResidual(Layer):
 class LinearAttention(Layer):
     """A recurrent layer of heads with a matrix each as their state: S_t = g S_(t-1) + k_t^T v_t, out_t = q_t S_t / sqrt(d),
     with q, k, v = x Wq^T, x Wk^T, x Wv^T and the heads' decays g = sigmoid(decay). No counterpart in the reference
-    (the Lstm layer's relative); needs a handler with linear_attention_forward."""
+    (the Lstm layer's relative); needs a handler with linear_attention_forward. Heads have at most 128 features. All
+    sequences start from a state of zeros and last to the last step: lengths, carried states and single steps are to be
+    had from the handler's methods."""
+
+    MOST_FEATURES = 128        # of a head: what the handler's operator takes
 
     def __init__(self, size, heads):
         self.size = int(size)
         self.heads = int(heads)
-        if self.size % self.heads:
+        if self.heads < 1 or self.size < 1 or self.size % self.heads:
             raise ValueError("%d features are not those of %d heads" % (self.size, self.heads))
+        if self.size // self.heads > self.MOST_FEATURES:
+            raise ValueError("heads of %d features; %d are the most" % (self.size // self.heads, self.MOST_FEATURES))
         self.scale = (self.size // self.heads) ** -0.5
 
     def setup(self, in_shapes):

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from brainstorm_amd.drivers import configs
-from brainstorm_amd.drivers.layers import FullyConnected, GatedResidual, Input, Loss, Lstm, SoftmaxCE
+from brainstorm_amd.drivers.layers import FullyConnected, GatedResidual, Input, LinearAttention, Loss, Lstm, SoftmaxCE
 from brainstorm_amd.drivers.net import MomentumStepper, Net, OrthogonalStepper
 from oracle.sequence_ops import SequenceRefHandler
 
@@ -279,3 +279,10 @@ def test_inputs_from_one_recurrent_output_on_the_gpu(hip, inputs):
     for name, (a, b, _) in got[1][1].items():
         want = got[1][0][a:b]
         assert np.abs(got[0][0][a:b] - want).max() <= 2e-4 * np.abs(want).max(), name
+
+
+def test_heads_that_the_operator_does_not_take_are_refused_by_the_layer():
+    assert LinearAttention(1024, 8).scale == 128 ** -0.5
+    for size, heads in ((1032, 8), (129, 1), (10, 3), (0, 2), (8, 0), (-8, -2)):
+        with pytest.raises(ValueError):
+            LinearAttention(size, heads)
