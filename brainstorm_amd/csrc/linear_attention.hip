@@ -573,7 +573,8 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
             a.out[(p * a.batch * a.heads + bh) * a.dj + j] = 0.0f;
     // the workgroup of the segment with the last position has the final state
     const bool last = len > 0 ? (pe == len && pe > p0) : seg == 0;
-    if (last && (a.fin || (TAN && a.dfin))) {
+    const bool moved = len > 0;            // an empty sequence's state is the one it had, whatever the decay
+    if (last && (a.fin || (TAN && a.dfin && moved))) {
 #pragma unroll
         for (int it = 0; it < NI; ++it)
 #pragma unroll
@@ -582,7 +583,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 if (i >= a.di || j >= a.dj) continue;
                 const int64_t at = bh * per_state + i * a.si + j * a.sj;
                 if (a.fin) a.fin[at] = c[it][r];
-                if (TAN && a.dfin) slope += static_cast<double>(a.dfin[at]) * dc[it][r];
+                if (TAN && a.dfin && moved) slope += static_cast<double>(a.dfin[at]) * dc[it][r];
             }
     }
     if constexpr (TAN) {

@@ -509,3 +509,16 @@ def test_a_state_replaced_by_several_segments(hip, shape):
     for n, (x, name) in enumerate(zip(grads + [up["dnew"]], ("dq", "dk", "dv", "dstate"))):
         n = 4 if name == "dstate" else n
         close(x.get(), want[n], size[n], roundings(time, max(dk, dv)), name)
+
+
+@pytest.mark.parametrize("time", [2, 40, 300])
+def test_an_empty_sequence_adds_nothing_to_the_gradient_of_the_decay(hip, time):
+    # its new state is its state, whatever the decay: also where the gradient from behind is not finite
+    a = inputs(63, time, 3, 2, 12, 16)
+    a["lengths"] = np.array([time, 0, time // 2], F32)
+    clean = backward(hip, a, True)
+    a["dnew"][1, 0, 3, 4], a["dnew"][1, 1, 5, 6] = np.inf, np.nan
+    got = backward(hip, a, True)
+    for n in range(4):
+        assert_bit_equal(got[n], clean[n])
+    assert_bit_equal(got[4], np.stack([clean[4][0], a["dnew"][1], clean[4][2]]))
