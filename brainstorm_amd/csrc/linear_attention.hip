@@ -81,6 +81,12 @@ __device__ __forceinline__ double power(double g, int64_t n) {
     return r;
 }
 
+// c behind n steps of decay g, w = g^n. An infinite one stays infinite where its power has become 0.
+template <class T>
+__device__ __forceinline__ T decayed(T w, T g, int64_t n, T c) {
+    return w == 0 && g != 0 && __builtin_isinf(c) ? (g < 0 && (n & 1) ? -c : c) : w * c;
+}
+
 // Steps of sequence b: lengths are float32 like the framework's labels, truncated; NaN counts as 0.
 __device__ __forceinline__ int64_t sequence_length(const float* lengths, int64_t b, int64_t time) {
     if (!lengths) return time;
@@ -148,7 +154,8 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
     __shared__ __attribute__((aligned(16))) float q_all[STATE ? 4 : 2 * kRows];
     __shared__ __attribute__((aligned(16))) float k_all[2 * kRows];
     __shared__ f4 score_s[STATE ? 1 : (TAN ? 6 : 3) * kWave];
-    __shared__ float pw[kChunk + 1], pl[kChunk + 1], sl[kChunk + 1];     // g^n, what its rounding left, n g^(n-1)
+    __shared__ float pw[kChunk + 1], sl[kChunk + 1];                     // g^n, n g^(n-1)
+    __shared__ float pt[kChunk + 1], pl[kChunk + 1];                     // g^n in two parts of the same sign
     __shared__ float pk[kChunk + 1], sk[kChunk + 1];                     // kv_scale times g^n and n g^(n-1)
     __shared__ double part_s[NW];
 
@@ -256,7 +263,10 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
     if (tid <= kChunk) {
         const double x = power(g, tid);
         pw[tid] = static_cast<float>(x);
-        pl[tid] = static_cast<float>(x - pw[tid]);
+        // The first part is one unit less than the rounded power, so that half a unit at least is left for the second and both
+        // have one sign: an infinite state stays one, where inf - inf or 0 inf would be NaN.
+        pt[tid] = pw[tid] != 0.0f ? __uint_as_float(__float_as_uint(pw[tid]) - 1) : 0.0f;
+        pl[tid] = static_cast<float>(x - pt[tid]);
         sl[tid] = tid ? static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
         pk[tid] = a.kv_scale * pw[tid];
         sk[tid] = a.kv_scale * sl[tid];
@@ -314,7 +324,9 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 }
                 read(u, slots + s * each, a.dj, 1);
 #pragma unroll
-                for (int it = 0; it < NI; ++it) c[it] = w * c[it] + u[it];
+                for (int it = 0; it < NI; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) c[it][r] = decayed(w, gf, steps, c[it][r]) + u[it][r];
             }
     }
     double slope = 0.0;
@@ -458,7 +470,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                     vw[bt][r] = pk[e > 0 ? e : 0] * v_r[bt][r];
                     if (TAN) vs[bt][r] = sk[e > 0 ? e : 0] * v_r[bt][r];
                 }
-            const float w = pw[m], wl = pl[m], dw = sl[m];
+            const float w = pt[m], wl = pl[m], dw = sl[m];
             {
                 float kf[2][8];
                 auto read = [&](int it) {
@@ -471,7 +483,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 for (int it = 0; it < NI; ++it) {
                     if (it + 1 < NI) read(it + 1);
                     one_step_ahead();
-                    // the power with what its rounding left: the same factor every 32 positions
+                    // the power in two parts: the same factor every 32 positions
                     if (TAN) dc[it] = w * dc[it] + (wl * dc[it] + dw * c[it]);
                     c[it] = w * c[it] + wl * c[it];
 #pragma unroll
@@ -976,13 +988,14 @@ __global__ __launch_bounds__(kBlock) void la_scan_kernel(Passes passes) {
                 slot[x * step] = static_cast<float>(c);
                 if (TAN) slot[x * step + per_state] = static_cast<float>(dc);
                 const int64_t left = len - static_cast<int64_t>(first + x) * a.seg_len;
+                const int64_t steps = left < 0 ? 0 : left < a.seg_len ? left : a.seg_len;
                 double w = full, dw = dfull;
                 if (left < a.seg_len) {
-                    w = power(g, left > 0 ? left : 0);
-                    dw = left > 0 ? left * power(g, left - 1) : 0.0;
+                    w = power(g, steps);
+                    dw = steps ? steps * power(g, steps - 1) : 0.0;
                 }
                 if (TAN) dc = w * dc + dw * c + du[x];
-                c = w * c + u[x];
+                c = decayed(w, g, steps, c) + u[x];
             }
             first += kScanned;
             slot += kScanned * step;

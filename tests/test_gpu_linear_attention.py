@@ -522,3 +522,60 @@ def test_an_empty_sequence_adds_nothing_to_the_gradient_of_the_decay(hip, time):
     for n in range(4):
         assert_bit_equal(got[n], clean[n])
     assert_bit_equal(got[4], np.stack([clean[4][0], a["dnew"][1], clean[4][2]]))
+
+
+def kinds(x):
+    """0 for finite elements, 1, -1 and 2 for infinities and NaN."""
+    return np.where(np.isnan(x), 2, np.where(np.isfinite(x), 0, np.sign(x)))
+
+
+@pytest.mark.parametrize("time,lengths", [(3, None), (20, None), (33, None), (64, (64, 40)), (100, (0, 100)), (300, (299, 65)),
+                                          (700, None), (700, (64, 130))])
+@pytest.mark.parametrize("decay", [[0.9, 1.0], [-0.5, 0.3], [0.07, -0.9]])
+def test_infinite_states_stay_infinite(hip, time, lengths, decay):
+    # infinities on their own in their rows and columns: sums with them are infinities of one sign, and so is what the
+    # recurrence makes of them; one sequence has a NaN as well
+    a = inputs(60, time, 2, 2, 20, 24)
+    a["decay"] = np.array(decay, F32)
+    a["lengths"] = None if lengths is None else np.array(lengths, F32)
+    for name in ("state", "dnew"):
+        a[name][0, 0, 3, 5], a[name][0, 1, 4, 6], a[name][1, 1, 7, 8] = np.inf, -np.inf, np.inf
+        a[name][1, 1, 9, 2] = np.nan
+    with np.errstate(invalid="ignore"):
+        want = list(ops.linear_attention(a["q"], a["k"], a["v"], a["decay"], 0.3, a["state"], a["lengths"]))
+        back = ops.linear_attention_gradients(a["q"], a["k"], a["v"], a["decay"], a["dout"], 0.3, a["state"], a["dnew"],
+                                              a["lengths"])
+    got = list(forward(hip, a, True)) + backward(hip, a, True)
+    want += list(back)
+    for x, w, name in zip(got, want, ("out", "new_state", "dq", "dk", "dv", "ddecay", "dstate")):
+        if name == "ddecay":                          # infinities of both signs meet in its sum
+            assert (np.isfinite(x) == np.isfinite(w)).all()
+        else:
+            assert (kinds(x) == kinds(w)).all(), "%s: %d elements" % (name, (kinds(x) != kinds(w)).sum())
+
+
+def test_infinite_states_behind_decays_that_have_vanished(hip):
+    # 0.5 to the power of a segment's steps is 0 in float32 and, over all segments, in float64
+    for time in (300, 1200, 8000):
+        a = inputs(61, time, 1, 1, 16, 64)
+        a["decay"][:] = 0.5
+        a["state"][0, 0, 3, 5] = np.inf
+        want, want_new = ops.linear_attention(a["q"], a["k"], a["v"], a["decay"], 0.3, a["state"])
+        out, new = forward(hip, a, True)
+        assert (kinds(out) == kinds(want)).all() and (kinds(new) == kinds(want_new)).all()
+        assert np.isposinf(new[0, 0, 3, 5])
+
+
+@pytest.mark.parametrize("time,at", [(3, 1), (40, 5), (40, 20), (128, 99), (200, 77), (600, 300)])
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("carry", [False, True])
+def test_exactly_the_positions_that_see_a_value_are_not_finite(hip, time, at, name, carry):
+    a = inputs(62, time, 2, 2, 20, 24)
+    a[name][at, 0, 3] = np.nan
+    a[name][at + 1, 0, 5] = np.inf
+    with np.errstate(invalid="ignore"):
+        want, want_new = ops.linear_attention(a["q"], a["k"], a["v"], a["decay"], 0.3, a["state"] if carry else None)
+    out, new = forward(hip, a, carry)
+    assert (np.isfinite(out) == np.isfinite(want)).all() and not np.isfinite(out).all()
+    if carry:
+        assert (np.isfinite(new) == np.isfinite(want_new)).all()
