@@ -37,6 +37,9 @@
 //   800 sequences of 100 steps of 125, all scores: forward 66 us, backward 168 us
 #include "common.h"
 
+#include <cfloat>
+#include <limits>
+
 #pragma clang fp contract(fast)
 
 namespace bship {
@@ -81,10 +84,12 @@ __device__ __forceinline__ double power(double g, int64_t n) {
     return r;
 }
 
-// c behind n steps of decay g, w = g^n. An infinite one stays infinite where its power has become 0.
+// x = g^n, rounded to T but to 0 only for g = 0: what it weighs has vanished all the same (T's least number is as near as
+// 0), but an infinite state stays infinite, as step by step.
 template <class T>
-__device__ __forceinline__ T decayed(T w, T g, int64_t n, T c) {
-    return w == 0 && g != 0 && __builtin_isinf(c) ? (g < 0 && (n & 1) ? -c : c) : w * c;
+__device__ __forceinline__ T not_vanished(double x, double g, int n) {
+    const T r = static_cast<T>(x);
+    return r != 0 || g == 0 ? r : g < 0 && (n & 1) ? -std::numeric_limits<T>::denorm_min() : std::numeric_limits<T>::denorm_min();
 }
 
 // Steps of sequence b: lengths are float32 like the framework's labels, truncated; NaN counts as 0.
@@ -262,11 +267,12 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
 
     if (tid <= kChunk) {
         const double x = power(g, tid);
-        pw[tid] = static_cast<float>(x);
+        pw[tid] = not_vanished<float>(x, g, tid);
         // The first part is one unit less than the rounded power, so that half a unit at least is left for the second and both
         // have one sign: an infinite state stays one, where inf - inf or 0 inf would be NaN.
-        pt[tid] = pw[tid] != 0.0f ? __uint_as_float(__float_as_uint(pw[tid]) - 1) : 0.0f;
-        pl[tid] = static_cast<float>(x - pt[tid]);
+        const bool normal = fabsf(pw[tid]) > FLT_MIN;
+        pt[tid] = normal ? __uint_as_float(__float_as_uint(pw[tid]) - 1) : pw[tid];
+        pl[tid] = not_vanished<float>(normal ? x - pt[tid] : 0.0, g, tid);
         sl[tid] = tid ? static_cast<float>(tid * power(g, tid - 1)) : 0.0f;
         pk[tid] = a.kv_scale * pw[tid];
         sk[tid] = a.kv_scale * sl[tid];
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
             for (int s = 0; s < seg; ++s) {
                 const int64_t rest = len - static_cast<int64_t>(s) * a.seg_len;
                 const int64_t steps = rest < 0 ? 0 : rest < a.seg_len ? rest : a.seg_len;
-                const float w = static_cast<float>(power(g, steps));
+                const float w = not_vanished<float>(power(g, steps), g, static_cast<int>(steps));
                 f4 u[NI];
                 if constexpr (TAN) {
                     const float dw = steps ? static_cast<float>(steps * power(g, steps - 1)) : 0.0f;
@@ -324,9 +330,7 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 }
                 read(u, slots + s * each, a.dj, 1);
 #pragma unroll
-                for (int it = 0; it < NI; ++it)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) c[it][r] = decayed(w, gf, steps, c[it][r]) + u[it][r];
+                for (int it = 0; it < NI; ++it) c[it] = w * c[it] + u[it];
             }
     }
     double slope = 0.0;
@@ -979,7 +983,11 @@ __global__ __launch_bounds__(kBlock) void la_scan_kernel(Passes passes) {
         };
         fetch(0);
         const int64_t len = sequence_length(a.lengths, bh / a.heads, a.time);
-        const double g = decay, full = power(g, a.seg_len), dfull = a.seg_len * power(g, a.seg_len - 1);
+        // segments before `whole` have all their positions, that one `rest` of them, those behind it none
+        const int whole = static_cast<int>(len) / a.seg_len, rest = static_cast<int>(len) % a.seg_len;
+        const double g = decay, full = not_vanished<double>(power(g, a.seg_len), g, a.seg_len);
+        const double part = not_vanished<double>(power(g, rest), g, rest);
+        const double dfull = a.seg_len * power(g, a.seg_len - 1), dpart = rest ? rest * power(g, rest - 1) : 0.0;
         double c = len > 0 && !a.reverse ? decay * init : init, dc = len > 0 ? init : 0.0f;
         for (int first = 0;;) {
 #pragma unroll
@@ -987,15 +995,10 @@ __global__ __launch_bounds__(kBlock) void la_scan_kernel(Passes passes) {
                 if (first + x >= a.segs) break;
                 slot[x * step] = static_cast<float>(c);
                 if (TAN) slot[x * step + per_state] = static_cast<float>(dc);
-                const int64_t left = len - static_cast<int64_t>(first + x) * a.seg_len;
-                const int64_t steps = left < 0 ? 0 : left < a.seg_len ? left : a.seg_len;
-                double w = full, dw = dfull;
-                if (left < a.seg_len) {
-                    w = power(g, steps);
-                    dw = steps ? steps * power(g, steps - 1) : 0.0;
-                }
+                const double w = first + x < whole ? full : first + x == whole ? part : 1.0;
+                const double dw = first + x < whole ? dfull : first + x == whole ? dpart : 0.0;
                 if (TAN) dc = w * dc + dw * c + du[x];
-                c = decayed(w, g, steps, c) + u[x];
+                c = w * c + u[x];
             }
             first += kScanned;
             slot += kScanned * step;

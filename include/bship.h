@@ -711,8 +711,7 @@ int bship_fusing_stats(unsigned long long* calls, unsigned long long* unfused,
  * and out is 0 there. dk and dv are 1 to 128, and batch * heads * max(dk, dv) is at most 2^25 (a time step of 128 MiB) for
  * more than 3 steps and for gradients, else BSHIP_ERR_UNSUPPORTED with nothing launched.
  * A value that is not finite reaches the outputs of its own and later positions only; an infinite entry of
- * the state stays infinite for |decay| >= 0.07 (below, a chunk's power of the decay underflows and it may
- * become NaN, as it does for a decay of 0). out may not overlap an input. Products and sums are float32. Takes scratch from the pool; recordable. */
+ * the state stays infinite unless the decay is 0. out may not overlap an input. Products and sums are float32. Takes scratch from the pool; recordable. */
 int bship_linear_attention_fwd_f32(const float* q, const float* k, const float* v,
                                    const float* decay, const float* lengths, const float* state,
                                    float* out, float* new_state, int64_t time, int64_t batch,

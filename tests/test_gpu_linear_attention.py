@@ -531,7 +531,7 @@ def kinds(x):
 
 @pytest.mark.parametrize("time,lengths", [(3, None), (20, None), (33, None), (64, (64, 40)), (100, (0, 100)), (300, (299, 65)),
                                           (700, None), (700, (64, 130))])
-@pytest.mark.parametrize("decay", [[0.9, 1.0], [-0.5, 0.3], [0.07, -0.9]])
+@pytest.mark.parametrize("decay", [[0.9, 1.0], [-0.5, 0.3], [0.07, -0.9], [1e-3, -1e-20]])
 def test_infinite_states_stay_infinite(hip, time, lengths, decay):
     # infinities on their own in their rows and columns: sums with them are infinities of one sign, and so is what the
     # recurrence makes of them; one sequence has a NaN as well
@@ -555,15 +555,15 @@ def test_infinite_states_stay_infinite(hip, time, lengths, decay):
 
 
 def test_infinite_states_behind_decays_that_have_vanished(hip):
-    # 0.5 to the power of a segment's steps is 0 in float32 and, over all segments, in float64
-    for time in (300, 1200, 8000):
+    # 0.5 to the power of a segment's steps is 0 in float32 and, over all segments, in float64; 0.01 to that of a chunk's
+    for time, decay in ((300, 0.5), (1200, 0.5), (8000, 0.5), (70, 0.01), (700, -0.01)):
         a = inputs(61, time, 1, 1, 16, 64)
-        a["decay"][:] = 0.5
+        a["decay"][:] = decay
         a["state"][0, 0, 3, 5] = np.inf
         want, want_new = ops.linear_attention(a["q"], a["k"], a["v"], a["decay"], 0.3, a["state"])
         out, new = forward(hip, a, True)
         assert (kinds(out) == kinds(want)).all() and (kinds(new) == kinds(want_new)).all()
-        assert np.isposinf(new[0, 0, 3, 5])
+        assert np.isinf(new[0, 0, 3, 5])
 
 
 @pytest.mark.parametrize("time,at", [(3, 1), (40, 5), (40, 20), (128, 99), (200, 77), (600, 300)])
