@@ -463,7 +463,15 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 }
             }
         }
-        // C = g^m C + sum_b g^(m-b) k_b^T v_b
+        // C = g^m C + sum_b g^(m-b) k_b^T v_b. A chunk's products are summed apart and added once: onto the state itself each would
+        // round against its magnitude. The sum is added behind other products, which run while it comes. It begins with the
+        // smaller part of the power, w + wl: the same factor every 32 positions.
+        const float w = pt[m], wl = pl[m], dw = sl[m];
+        f4 u[2], du[2];
+        auto add = [&](int it) {
+            if (TAN) dc[it] = w * dc[it] + (dw * c[it] + du[it & 1]);
+            c[it] = w * c[it] + u[it & 1];
+        };
         if (mine) {
             float vw[2][4], vs[2][4];
 #pragma unroll
@@ -474,7 +482,6 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                     vw[bt][r] = pk[e > 0 ? e : 0] * v_r[bt][r];
                     if (TAN) vs[bt][r] = sk[e > 0 ? e : 0] * v_r[bt][r];
                 }
-            const float w = pt[m], wl = pl[m], dw = sl[m];
             {
                 float kf[2][8];
                 auto read = [&](int it) {
@@ -487,15 +494,16 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 for (int it = 0; it < NI; ++it) {
                     if (it + 1 < NI) read(it + 1);
                     one_step_ahead();
-                    // the power in two parts: the same factor every 32 positions
-                    if (TAN) dc[it] = w * dc[it] + (wl * dc[it] + dw * c[it]);
-                    c[it] = w * c[it] + wl * c[it];
+                    u[it & 1] = wl * c[it];
+                    if (TAN) du[it & 1] = wl * dc[it];
 #pragma unroll
                     for (int x = 0; x < 4 * kTiles; ++x) {
-                        c[it] = mfma(kf[it & 1][x], vw[x >> 2][x & 3], c[it]);
-                        if (TAN) dc[it] = mfma(kf[it & 1][x], vs[x >> 2][x & 3], dc[it]);
+                        u[it & 1] = mfma(kf[it & 1][x], vw[x >> 2][x & 3], u[it & 1]);
+                        if (TAN) du[it & 1] = mfma(kf[it & 1][x], vs[x >> 2][x & 3], du[it & 1]);
                     }
+                    if (it > 0) add(it - 1);
                 }
+                if constexpr (STATE) add(NI - 1);
             }
         }
         if constexpr (!STATE) {
@@ -514,11 +522,11 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 for (int bt = 0; bt < kTiles; ++bt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v_r[bt][r] = __builtin_isfinite(v_r[bt][r]) ? v_r[bt][r] : 0.0f;
-            f4 w[3], dw[3];
+            f4 ws[3], dws[3];
 #pragma unroll
             for (int tile = 0; tile < (kTiles == 2 ? 3 : 1); ++tile) {
-                w[tile] = score_s[tile * kWave + lane];
-                if (TAN) dw[tile] = score_s[(3 + tile) * kWave + lane];
+                ws[tile] = score_s[tile * kWave + lane];
+                if (TAN) dws[tile] = score_s[(3 + tile) * kWave + lane];
             }
 #pragma unroll
             for (int bt = 0; bt < kTiles; ++bt)
@@ -526,9 +534,10 @@ __global__ __launch_bounds__(NW * kWave, NW == 8 ? (TAN ? 2 : 4) : NI > 4 ? 2 : 
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int at = bt; at < kTiles; ++at) {
-                        o[at] = mfma(v_r[bt][r], w[bt + at][r], o[at]);
-                        if (TAN) dz[at] = mfma(v_r[bt][r], dw[bt + at][r], dz[at]);
+                        o[at] = mfma(v_r[bt][r], ws[bt + at][r], o[at]);
+                        if (TAN) dz[at] = mfma(v_r[bt][r], dws[bt + at][r], dz[at]);
                     }
+            add(NI - 1);
             const int left = a.dj - j0 - 4 * lq;
             if (!all_finite) {
                 const float* here = v - move_j;

@@ -579,3 +579,25 @@ def test_exactly_the_positions_that_see_a_value_are_not_finite(hip, time, at, na
     assert (np.isfinite(out) == np.isfinite(want)).all() and not np.isfinite(out).all()
     if carry:
         assert (np.isfinite(new) == np.isfinite(want_new)).all()
+
+
+def test_a_long_memory_loses_no_more_than_one_rounding_a_chunk(hip):
+    # A state that remembers 4096 positions, formed in one piece. Every 32 positions it is multiplied and added to with one
+    # rounding of its own size; what is added is a sum of 32 products with random signs, whose additions round against partial
+    # sums of half its square in the mean, and two roundings of each product. A rounding's square is at most u^2 / 3 in the mean, what
+    # is added makes up the state's square, and an old error fades with the state: the relative square of the error is at most
+    # u^2 / 3 (sum over chunks of g^(2 32 c) + 32 / 2 + 2 + 2), the last 2 for the decay's powers.
+    time, batch, heads, d = 4096, 40, 8, 16
+    rng = np.random.RandomState(70)
+    q, k, v = (rng.standard_normal((time, batch, heads * d)).astype(F32) for _ in range(3))
+    decay = np.full(heads, 1 - 2.0 ** -12, F32)
+    up = [hip.create_from_numpy(x) for x in (q, k, v, decay)]
+    new = hip.ones((batch, heads, d, d))
+    hip.linear_attention_forward(*up, hip.empty(v.shape), new_state=new)
+    want = np.zeros((batch, heads, d, d))
+    kf, vf = (x.reshape(time, batch, heads, d).astype(np.float64) for x in (k, v))
+    for t in range(time):
+        want = float(decay[0]) * want + kf[t, :, :, :, None] * vf[t, :, :, None, :]
+    passed = (float(decay[0]) ** (64.0 * np.arange(time // 32))).sum()
+    off = np.linalg.norm(new.get() - want) / np.linalg.norm(want)
+    assert off <= U * np.sqrt((passed + 20) / 3)
