@@ -5,6 +5,7 @@ import gc
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -16,6 +17,8 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+    # an exception that ends a thread fails the test that started it: what the thread should have found wrong is not found
+    config.addinivalue_line("filterwarnings", "error::pytest.PytestUnhandledThreadExceptionWarning")
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -23,6 +26,15 @@ def earlier_garbage():
     """Collects what the tests of other files left in cycles, handlers above all. Collected in the middle of a test they
     release their generators, which enqueues what the fusing window holds, and some tests count its launches."""
     gc.collect()
+
+
+@pytest.fixture(autouse=True)
+def threads_end():
+    """No thread that a test started is left when it ends: a join that timed out is a thread that hangs."""
+    before = set(threading.enumerate())
+    yield
+    left = [t.name for t in threading.enumerate() if t not in before and not t.daemon]
+    assert not left, "threads that the test started still run: %s" % left
 
 
 @pytest.fixture(scope="session")
