@@ -204,3 +204,69 @@ def test_small_matrices_lose_no_more_than_float32(hip):
         here.append(off(out.get(), want))
         there.append(off(plain(m), want))
     assert np.mean(here) <= 1.2 * np.mean(there), (np.mean(here), np.mean(there))
+
+
+# How near the same steps in float32 the kernels have to be. Both lose bits where a matrix is stored and where products are added
+# up, and the steps treat both alike. Stored: float32 rounds to 2^-24 of the binade, evenly spread, a mean square of 2^-48 / 3; two
+# float16 planes round to half a unit of the low one, whose values spread evenly over its binades: 2^-46 / 3 (1/2 + 1/8 + ...) =
+# (8/3) 2^-48 / 3. The product of two low planes that is left out: the square of a mean square of 2^-22 / 3, 2^-44 / 9, against the
+# 2 2^-48 / 3 of two rounded factors another 8/3. Together 16/3, the root of which is 2.3; added up are 32 products at a time, where
+# float32 rounds after each. 3 bounds the ratio then. Matrices of a few entries can be lucky in float32: a step's own error is
+# about 30 2^-23 at most (A to 4.4 2^-23, p to 4.8 times that and 3.5 2^-23, the product to 1.2 times that), a quarter of it with signs
+# at random, 2^-20.
+def float32_steps(m, steps=5):
+    if m.ndim == 3:
+        return np.stack([float32_steps(x, steps) for x in m])
+    x = (m.astype(np.float64) / np.linalg.norm(m.astype(np.float64))).astype(F32)
+    x = x.T if x.shape[0] > x.shape[1] else x
+    for _ in range(steps):
+        gram = x @ x.T
+        x = F32(3.4445) * x + (F32(-4.7750) * gram + F32(2.0315) * (gram @ gram)) @ x
+    return x.T if m.shape[0] > m.shape[1] else x
+
+
+def near_float32(hip, m, steps=5):
+    out = hip.ones(m.shape)
+    hip.orthogonalize(hip.create_from_numpy(m), out, steps=steps)
+    want = ops.orthogonalize(m, steps)
+    here, there = off(out.get(), want), off(float32_steps(m, steps), want)
+    assert here <= 3 * there + 2.0 ** -20, (here, there)
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES + [(8, 2400), (2400, 64), (127, 131), (192, 192), (257, 1025)])
+def test_as_near_as_float32(hip, rows, cols):
+    near_float32(hip, matrix(rows * 7 + cols, rows, cols))
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 8, 12])
+@pytest.mark.parametrize("shape", [(40, 70), (200, 150)])
+def test_other_numbers_of_steps_as_near_as_float32(hip, steps, shape):
+    near_float32(hip, matrix(3, *shape), steps)
+
+
+@pytest.mark.parametrize("shape", [(4, 30, 50), (3, 140, 60), (2, 256, 384), (4, 300, 300)])
+def test_stacks_as_near_as_float32(hip, shape):
+    near_float32(hip, matrix(4, *shape))
+
+
+def test_low_rank_and_uneven_matrices_as_near_as_float32(hip):
+    rng = np.random.RandomState(6)
+    one = np.zeros((130, 70), F32)
+    one[100, 5] = -3.0
+    spiked = matrix(7, 100, 260)
+    spiked[3] *= 1e4
+    for m in ((rng.standard_normal((200, 3)) @ rng.standard_normal((3, 150))).astype(F32), one, spiked):
+        near_float32(hip, m)
+
+
+@pytest.mark.parametrize("shape", [(12, 20), (200, 30), (3, 64, 65), (1000, 205)])
+def test_update_as_near_as_float32(hip, shape):
+    g, v, p = matrix(11, *shape), matrix(12, *shape), np.zeros(shape, F32)
+    dg, dv, dp = (hip.create_from_numpy(x) for x in (g, v, p))
+    hip.orthogonal_update(0.9, -0.5, dg, dv, dp)
+    v = F32(0.9) * v + g                             # two roundings each, as the handler's own operations
+    u = g + F32(0.9) * v
+    factor = -0.5 * np.sqrt(max(1.0, shape[-2] / shape[-1]))
+    want = factor * ops.orthogonalize(u)
+    here, there = off(dp.get(), want), off(float32_steps(u), ops.orthogonalize(u))
+    assert here <= 3 * there + 2.0 ** -20 + 2.0 ** -23, (here, there)      # the factor and the sum round too
