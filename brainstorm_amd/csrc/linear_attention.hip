@@ -21,7 +21,7 @@
 // positions (a, b local positions):
 //   o_a    = out_scale (g^a q_a C + sum_{b<=a} g^(a-b) (q_a . k_b) v_b)
 //   C_next = g^n C + sum_b g^(n-b) k_b^T v_b
-// Powers come from a table made by repeated squaring in float64, so every decay is allowed, 0 and 1 included.
+// Powers come from a table made by repeated squaring in float64, so every decay is allowed whose powers float32 holds, 0 and 1 included.
 //
 // The gradient of the decay is the sum over (t, s) of (t-s) g^(t-s-1) scale (q_t.k_s)(do_t.v_s). It is taken
 // in the dq pass by carrying the derivative C' of the state by g beside the state (C'_next = g^n C' +

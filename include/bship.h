@@ -703,8 +703,9 @@ int bship_fusing_stats(unsigned long long* calls, unsigned long long* unfused,
 /* Linear attention with a decay for each head, a recurrent layer's whole sequence:
  *     S_t = decay[h] S_(t-1) + k_t^T v_t,    out_t = scale q_t S_t
  * for every batch element and head. q, k are (time, batch, heads * dk), v and out (time, batch,
- * heads * dv), a head's features side by side; decay is (heads), any finite values (0 keeps the
- * position itself only, 1 forgets nothing); state, S before the first step, is (batch, heads, dk, dv)
+ * heads * dv), a head's features side by side; decay is (heads), 0 (keeps the position itself only)
+ * to 1 (forgets nothing), below 0 and beyond 1 too as long as float32 holds time * |decay|^time
+ * (where it does not, outputs may be NaN although the steps one by one would not overflow); state, S before the first step, is (batch, heads, dk, dv)
  * or NULL for zeros; new_state receives S behind the last step (NULL: not wanted) and may be state.
  * lengths (batch) or NULL: the steps of each batch element, float32 like all labels, truncated and
  * taken into [0, time] (NaN: 0); rows at and behind a length are neither read nor added to the state,

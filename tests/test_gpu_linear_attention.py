@@ -601,3 +601,15 @@ def test_a_long_memory_loses_no_more_than_one_rounding_a_chunk(hip):
     passed = (float(decay[0]) ** (64.0 * np.arange(time // 32))).sum()
     off = np.linalg.norm(new.get() - want) / np.linalg.norm(want)
     assert off <= U * np.sqrt((passed + 20) / 3)
+
+
+@pytest.mark.parametrize("shape,decay", [((100, 2, 2, 20, 24), [1.9, -1.5]), ((100, 2, 2, 100, 60), [-1.9, 1.2]),
+                                         ((40, 2, 2, 8, 8), [3.0, -6.0]), ((300, 2, 2, 20, 72), [1.25, -1.2]),
+                                         ((3, 2, 2, 8, 8), [1e6, -1e12])])
+@pytest.mark.parametrize("carry", [False, True])
+def test_decays_that_grow(hip, shape, decay, carry):
+    # as far as float32 holds the number of steps times the power of the decay
+    a = inputs(sum(shape) + 80, *shape)
+    a["decay"] = np.array(decay, F32)
+    check_forward(hip, a, carry)
+    check_backward(hip, a, carry)
