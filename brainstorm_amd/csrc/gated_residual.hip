@@ -8,7 +8,8 @@
 // backward (the row's two means are formed again, which costs two reductions and no memory). Memory bounds both: 10000 x
 // 1000 forward 38 us (5.3 TB/s), backward 58 us (5.5 TB/s) and 7 us for the weights' sums, 2048 x 4096 forward 30 us (5.6
 // TB/s; a large copy: 5.1). One vector of four columns per thread keeps enough rows under way: four per thread on a
-// wavefront per row took 51 and 115 us. The gate, the second norm, and the block itself (only the norm: h = pre * x / rms(x)) can be left out.
+// wavefront per row took 51 and 115 us. The gate, the second norm, and the block itself (only the norm: h = pre * x / rms(x),
+// 10000 x 1000: 14 us, its gradients 22 and 6) can be left out.
 #include "common.h"
 
 #pragma clang fp contract(fast)

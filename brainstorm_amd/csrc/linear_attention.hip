@@ -30,9 +30,9 @@
 //
 // What bounds it and what it takes (a large copy moves 5.1 TB/s on this card, a float32 product reaches 152 TFLOP/s):
 //   one step, 4096 sequences of 128 x 128: the state in and out, 537 MB: 106 us, 5.1 TB/s; 8 sequences: a launch, 3.7 us
-//   16 sequences of 8192 steps of 64: 70 us in three launches (states of the segments 22, scan 6, pass 45); 134 MB would
+//   16 sequences of 8192 steps of 64: 70 us in three launches (states of the segments 22, scan 6, pass 46); 134 MB would
 //     take 26 us, but a segment's chunks wait for each other
-//   128 sequences of 1024 steps of 128: forward 153 us, backward 464; 30 GFLOP that cannot be left out take 198 us; matrix
+//   128 sequences of 1024 steps of 128: forward 151 us, backward 484; 30 GFLOP that cannot be left out take 198 us; matrix
 //     cores 44 % (one wavefront a SIMD) to 55 % (two) busy, a quarter of the work is the derivative by the decay
 //   800 sequences of 100 steps of 125, all scores: forward 66 us, backward 168 us
 #include "common.h"
