@@ -21,7 +21,8 @@
 // positions (a, b local positions):
 //   o_a    = out_scale (g^a q_a C + sum_{b<=a} g^(a-b) (q_a . k_b) v_b)
 //   C_next = g^n C + sum_b g^(n-b) k_b^T v_b
-// Powers come from a table made by repeated squaring in float64, so every decay is allowed whose powers float32 holds, 0 and 1 included.
+// Powers come from a table made by repeated squaring in float64, so every decay is allowed whose powers float32 holds,
+// 0 and 1 included.
 //
 // The gradient of the decay is the sum over (t, s) of (t-s) g^(t-s-1) scale (q_t.k_s)(do_t.v_s). It is taken
 // in the dq pass by carrying the derivative C' of the state by g beside the state (C'_next = g^n C' +
@@ -89,7 +90,8 @@ __device__ __forceinline__ double power(double g, int64_t n) {
 template <class T>
 __device__ __forceinline__ T not_vanished(double x, double g, int n) {
     const T r = static_cast<T>(x);
-    return r != 0 || g == 0 ? r : g < 0 && (n & 1) ? -std::numeric_limits<T>::denorm_min() : std::numeric_limits<T>::denorm_min();
+    constexpr T least = std::numeric_limits<T>::denorm_min();
+    return r != 0 || g == 0 ? r : g < 0 && (n & 1) ? -least : least;
 }
 
 // Steps of sequence b: lengths are float32 like the framework's labels, truncated; NaN counts as 0.

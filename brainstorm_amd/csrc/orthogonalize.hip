@@ -442,8 +442,9 @@ constexpr int kFineMost = 128;      // matrices with smaller sides up to it take
 // The tile side: what 32 entries of the summed axis cost with one tile on every compute unit, in hundredths of a
 // microsecond, times the rounds that the tiles take. Measured (4096 x 4096: 256 against 192 and 128 for the full product
 // 336, 440 and 412 us, for the symmetric ones 280, 208 and 315; 4 x 1000 x 1000: 128 against 64 for the full product 34.5
-// and 38.7 us, for the symmetric ones 28.9 and 26.5); between the two a choice may be off, at a cost in time only. Tiles of 64 share a compute unit, so their rounds need not be
-// whole; where there is at most one for each, four groups share its summed axis (784 x 1200: 13 us, one group 20).
+// and 38.7 us, for the symmetric ones 28.9 and 26.5); between the two a choice may be off, at a cost in time only. Tiles of 64
+// share a compute unit, so their rounds need not be whole; where there is at most one for each, four groups share its summed
+// axis (784 x 1200: 13 us, one group 20).
 template <int MODE>
 int launch_product(ProductArgs a, unsigned count) {
     const bool fine = a.used_p <= kFineMost;            // the smaller side

@@ -1458,9 +1458,10 @@ class HipHandler(Handler):
     def linear_attention_forward(self, q, k, v, decay, out, scale=1.0, state=None, new_state=None, lengths=None):
         """Linear attention with a decay for each head over a whole sequence: S_t = decay S_(t-1) + k_t^T v_t,
         out_t = scale q_t S_t. q, k are (time, batch, heads * dk), v and out (time, batch, heads * dv), decay
-        (heads; usually 0 to 1, time * |decay| ** time has to be a float32), dk and dv at most 128. state (batch, heads, dk, dv) is S before the first step (None: zeros),
-        new_state receives S behind the last one and may be state. lengths (batch elements, like labels) gives
-        the steps of each: rows from there on are not read, out is 0 there."""
+        (heads; usually 0 to 1, time * |decay| ** time has to be a float32), dk and dv at most 128. state (batch,
+        heads, dk, dv) is S before the first step (None: zeros), new_state receives S behind the last one and may be
+        state. lengths (batch elements, like labels) gives the steps of each: rows from there on are not read, out
+        is 0 there."""
         sizes = self._attention_shapes("linear_attention_forward", q, k, v, decay, 2, (state, new_state), lengths,
                                        ((out, v),))
         shared = ((new_state, state),) if new_state is not None and state is not None and new_state.ptr == state.ptr else ()

@@ -730,7 +730,7 @@ int bship_linear_attention_bwd_f32(const float* q, const float* k, const float* 
 
 /* The norms around a block with its gate and residual scale, over (rows, width) matrices:
  *     y = residual_scale x + act(gate) * post * block / rms(block),    h = pre * y / rms(y),
- *     rms(v) = sqrt(mean(v * v) + epsilon) over a row
+ *     rms(v) = sqrt(mean(v * v) + epsilon) over a row, in float32: values beyond 1e19 count as infinite
  * act is a BSHIP_ACT_* code, BSHIP_ACT_SWISH included. gate NULL: no gate. pre NULL: no norm behind, h
  * is not written. block NULL: only the norm, h = pre * x / rms(x), y is not written. An output may be
  * block, gate or x, but neither the other output nor anything else that overlaps an operand. Recordable. */
